@@ -235,6 +235,35 @@ int nd_gated_residual_bwd_add(int dtype, const void* dy, const void* dres, const
                               void* dsum, void* dbranch, float* dgate_partials, int64_t rows, int64_t row_start,
                               int64_t seq_len, int64_t hidden, int64_t tile_rows, void* stream);
 
+/* -------------------------------------------------------------------- rotary positions */
+
+/* y = x with the first 2 * pairs dimensions of every head rotated: pair p of token (b, s) turns by
+ * t = positions[b, s, p / (pairs / axes)] * freqs[p] radians,
+ *   (a, b) -> (factor * (a cos t - b sin t), factor * (a sin t + b cos t)),
+ * a pair being elements (p, p + pairs) of the head, or (2p, 2p + 1) when `interleaved`; the rest of the head is copied.
+ * x [batch, seq_len, heads, head_dim] with element strides stride_b / stride_s / stride_h and contiguous head
+ * dimensions, y contiguous; ND_F16, ND_BF16 or ND_F32, fp32 arithmetic, one rounding. positions: pos_bytes (4 or 8)
+ * byte integers, `axes` per token, samples pos_stride_b elements apart (0: one set for all samples), any value
+ * (negative too): position * frequency is reduced modulo a turn exactly. freqs: [axes, pairs / axes] doubles on the
+ * device, row a belongs to axis a. inverse != 0 turns the other way: the gradient of x is nd_rotary of the gradient of y
+ * with inverse = 1 and the same factor. Interleaved pairs need an even head_dim when they are not 8-byte (16-bit types:
+ * 4-byte) aligned. No counterpart in the reference. */
+int nd_rotary(int dtype, const void* x, void* y, int64_t batch, int64_t seq_len, int64_t heads, int64_t head_dim,
+              int64_t stride_b, int64_t stride_s, int64_t stride_h, const void* positions, int pos_bytes,
+              int64_t pos_stride_b, const double* freqs, int64_t pairs, int64_t axes, int interleaved, float factor,
+              int inverse, void* stream);
+
+/* nd_qkv_pack_fwd with q and k rotated on the way (v is copied), and its backward: dq and dk turned back while dqkv is
+ * put together. qkv [batch, seq_len, 3 * heads * head_dim], q / k / v [batch, seq_len, heads, head_dim], all
+ * contiguous; the other arguments as in nd_rotary. */
+int nd_qkv_pack_rotary_fwd(int dtype, const void* qkv, void* q, void* k, void* v, int64_t batch, int64_t seq_len,
+                           int64_t heads, int64_t head_dim, const void* positions, int pos_bytes, int64_t pos_stride_b,
+                           const double* freqs, int64_t pairs, int64_t axes, int interleaved, float factor, void* stream);
+int nd_qkv_pack_rotary_bwd(int dtype, const void* dq, const void* dk, const void* dv, void* dqkv, int64_t batch,
+                           int64_t seq_len, int64_t heads, int64_t head_dim, const void* positions, int pos_bytes,
+                           int64_t pos_stride_b, const double* freqs, int64_t pairs, int64_t axes, int interleaved,
+                           float factor, void* stream);
+
 /* -------------------------------------------------------------------- FC1 */
 
 /* z = (x @ w^T) * alpha + bias, x [m,k] and w [n,k] both K-contiguous (nn.Linear layout).

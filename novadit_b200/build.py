@@ -41,6 +41,7 @@ CU_SOURCES = [
     "norm_f32.cu",
     "gate_act.cu",
     "rowops.cu",
+    "rotary.cu",
     "quant.cu",
     "fc1.cu",
     "noalloc.cu",

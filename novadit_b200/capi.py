@@ -67,6 +67,12 @@ SIGNATURES = {
     "nd_out_residual_fwd": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p]),
     "nd_qkv_pack_fwd": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p]),
     "nd_qkv_pack_bwd": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p]),
+    "nd_rotary": (c_int, [c_int, c_void_p, c_void_p, *[c_int64] * 7, c_void_p, c_int, c_int64, c_void_p, c_int64, c_int64,
+                          c_int, c_float, c_int, c_void_p]),
+    "nd_qkv_pack_rotary_fwd": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, *[c_int64] * 4, c_void_p, c_int,
+                                       c_int64, c_void_p, c_int64, c_int64, c_int, c_float, c_void_p]),
+    "nd_qkv_pack_rotary_bwd": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, *[c_int64] * 4, c_void_p, c_int,
+                                       c_int64, c_void_p, c_int64, c_int64, c_int, c_float, c_void_p]),
     "nd_gated_residual_fwd": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, *_SHAPE4, c_void_p]),
     "nd_gated_residual_ws_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int64]),
     "nd_adaln_fwd_residual": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -489,3 +495,17 @@ def quantize_e4m3(x):
     check(L.nd_quant_e4m3(DTYPE_IDS[x.dtype], _ptr(x), x.numel(), _ptr(amax), _ptr(q), _ptr(scale), st),
           "nd_quant_e4m3")
     return q, scale
+
+
+# ---------------------------------------------------------------- rotary positions
+def rotary(x, positions, freqs, *, interleaved=False, factor=1.0, inverse=False, y=None):
+    """`nd_rotary` on x [B, S, heads, D]; positions int32 / int64 [B, S(, axes)] or [S(, axes)], freqs float64."""
+    _need_cuda(x, positions, freqs)
+    b, s, h, d = x.shape
+    axes = freqs.shape[0] if freqs.dim() == 2 else 1
+    shared = positions.dim() == freqs.dim()
+    y = torch.empty_like(x) if y is None else y
+    check(lib().nd_rotary(DTYPE_IDS[x.dtype], _ptr(x), _ptr(y), b, s, h, d, s * h * d, h * d, d, _ptr(positions),
+                          positions.element_size(), 0 if shared else s * axes, _ptr(freqs), freqs.numel(), axes,
+                          int(interleaved), factor, int(inverse), _stream()), "rotary")
+    return y

@@ -1,0 +1,320 @@
+// Rotary positions (sm_100a): every pair (a, b) of a head's first 2 R dimensions becomes
+//   (f (a cos t - b sin t), f (a sin t + b cos t)),   t = position[axis of the pair] * freq[pair]
+// on a [B, S, heads, D] tensor, or on q and k while a fused projection [B, S, 3 heads D] is split into q, k, v (and on
+// the way back). The gradient is the same rotation by -t, so forward and backward share the kernel.
+//
+// The angle. t in radians as a 32-bit float is off by t * 2^-24, a tenth of a radian at position 10^6. Here a frequency
+// becomes a 64-bit fixed-point fraction of a turn, and position * fraction is ONE 64-bit integer product whose overflow
+// drops the whole turns: the remainder is exact, whatever the position. Its top 32 bits go to sincospi.
+//
+// Bound: HBM, one read and one write of every element (plus one position per token and axis). A CTA takes TT tokens:
+// it fills a table of TT x R (cos, sin) in shared memory once, and all heads (of q and k) read it, so a sine costs the
+// kernel 1 / heads of what it would cost per element. A thread then owns one vector slot of the token (a pair of
+// vectors R apart in the half layout, one vector of adjacent pairs in the interleaved one, a plain copy elsewhere) and
+// walks the TT tokens with it: the slot's address is decoded once, and the loads of the TT tokens are in flight together.
+#include "common.cuh"
+
+namespace nd {
+
+constexpr int kRotThreads = 256;
+constexpr int kRotTokens = 4;       // tokens per CTA
+constexpr int kRotMaxPairs = 1024;  // table of kRotTokens * pairs * 8 bytes = 32 KB at most
+
+struct RotSeg {  // one tensor of [tokens, heads, D]; strides in elements
+  const void* src;
+  void* dst;
+  long long src_b, src_s, src_h;
+  long long dst_b, dst_s, dst_h;
+  int rotate;
+};
+
+struct RotArgs {
+  RotSeg seg[3];
+  const void* positions;  // [B or 1, S, axes] of pos_bytes-byte integers, contiguous within a sample
+  const double* freqs;    // [axes, pairs / axes] radians per position
+  long long tokens, seq_len, pos_b;  // pos_b: elements between samples (0: shared)
+  int n_seg, heads, head_dim, pairs, axes, pos_bytes;
+  int rot_units, units;   // vector slots per head of a rotated segment: rotated ones, all
+  int copy_units;         // vector slots per head of a copied segment
+  unsigned units_mul, copy_mul;  // slot / units as a high product (0: units == 1)
+  float factor;
+  int inverse;
+};
+
+template <typename T, int V, bool ALIGNED> __device__ __forceinline__ void rot_load(Vec<T, V>& v, const T* p) {
+  if constexpr (ALIGNED) {
+    v.load_stream(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v.v[i] = p[i];
+  }
+}
+template <typename T, int V, bool ALIGNED> __device__ __forceinline__ void rot_store(const Vec<T, V>& v, T* p) {
+  if constexpr (ALIGNED) {
+    v.store(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) p[i] = v.v[i];
+  }
+}
+
+// the two products of a rotation, contracted the same way in every variant: the vector width never changes a result
+__device__ __forceinline__ float rot_re(float re, float im, float2 cs) { return fmaf(re, cs.x, -__fmul_rn(im, cs.y)); }
+__device__ __forceinline__ float rot_im(float re, float im, float2 cs) { return fmaf(re, cs.y, __fmul_rn(im, cs.x)); }
+
+// n / d for n < 2^16 and d < 2^16 with mul = ceil(2^32 / d): exact, since n * (mul * d - 2^32) < 2^32
+__device__ __forceinline__ int rot_div(int n, unsigned mul) {
+  return mul == 0 ? n : static_cast<int>(__umulhi(static_cast<unsigned>(n), mul));
+}
+
+template <typename T, int V, bool ALIGNED, bool INTERLEAVED>
+__global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotArgs a) {
+  extern __shared__ float2 table[];  // [kRotTokens][pairs]
+  __shared__ long long src_off[3][kRotTokens], dst_off[3][kRotTokens];
+  const long long t0 = static_cast<long long>(blockIdx.x) * kRotTokens;
+  const int nt = a.tokens - t0 < kRotTokens ? static_cast<int>(a.tokens - t0) : kRotTokens;
+  for (int i = threadIdx.x; i < a.n_seg * kRotTokens; i += blockDim.x) {
+    const int g = i / kRotTokens, j = i - g * kRotTokens;
+    if (j < nt) {
+      const long long b = (t0 + j) / a.seq_len, s = (t0 + j) - b * a.seq_len;
+      src_off[g][j] = b * a.seg[g].src_b + s * a.seg[g].src_s;
+      dst_off[g][j] = b * a.seg[g].dst_b + s * a.seg[g].dst_s;
+    }
+  }
+  const int per_axis = a.pairs / a.axes;
+  for (int i = threadIdx.x; i < nt * a.pairs; i += blockDim.x) {
+    const int j = i / a.pairs, p = i - j * a.pairs;
+    const long long b = (t0 + j) / a.seq_len, s = (t0 + j) - b * a.seq_len;
+    const long long at = b * a.pos_b + s * a.axes + p / per_axis;
+    const long long pos = a.pos_bytes == 8 ? __ldg(static_cast<const long long*>(a.positions) + at)
+                                           : static_cast<long long>(__ldg(static_cast<const int*>(a.positions) + at));
+    const double f = __ldg(a.freqs + p) * 0.15915494309189533576888376337251;  // turns per position
+    const unsigned long long frac = __double2ull_rz((f - floor(f)) * 18446744073709551616.0);
+    const unsigned long long turn = static_cast<unsigned long long>(pos) * frac;  // whole turns overflow away
+    float sn, cs;
+    sincospif(static_cast<float>(static_cast<int>(turn >> 32)) * 4.656612873077392578125e-10f, &sn, &cs);  // 2^-31
+    if (!isfinite(f)) sn = cs = __int_as_float(0x7fffffff);
+    table[i] = make_float2(cs * a.factor, (a.inverse ? -sn : sn) * a.factor);
+  }
+  __syncthreads();
+
+  for (int g = 0; g < a.n_seg; ++g) {
+    const RotSeg& sg = a.seg[g];
+    const int rot_units = sg.rotate ? a.rot_units : 0, units = sg.rotate ? a.units : a.copy_units;
+    const unsigned mul = sg.rotate ? a.units_mul : a.copy_mul;
+    const T* src = static_cast<const T*>(sg.src);
+    T* dst = static_cast<T*>(sg.dst);
+    for (int i = threadIdx.x; i < a.heads * units; i += blockDim.x) {
+      const int head = rot_div(i, mul), u = i - head * units;
+      const long long hs = head * sg.src_h, hd = head * sg.dst_h;
+      if (u < rot_units) {
+        if constexpr (INTERLEAVED) {
+          Vec<T, V> x[kRotTokens];
+#pragma unroll
+          for (int j = 0; j < kRotTokens; ++j)
+            if (j < nt) rot_load<T, V, ALIGNED>(x[j], src + src_off[g][j] + hs + u * V);
+#pragma unroll
+          for (int j = 0; j < kRotTokens; ++j) {
+            if (j >= nt) break;
+            float f[V];
+            x[j].unpack(f);
+#pragma unroll
+            for (int e = 0; e < V; e += 2) {
+              const float2 cs = table[j * a.pairs + (u * V + e) / 2];
+              const float re = f[e], im = f[e + 1];
+              f[e] = rot_re(re, im, cs);
+              f[e + 1] = rot_im(re, im, cs);
+            }
+            x[j].pack(f);
+            rot_store<T, V, ALIGNED>(x[j], dst + dst_off[g][j] + hd + u * V);
+          }
+        } else {
+          Vec<T, V> x[kRotTokens], y[kRotTokens];
+#pragma unroll
+          for (int j = 0; j < kRotTokens; ++j)
+            if (j < nt) {
+              rot_load<T, V, ALIGNED>(x[j], src + src_off[g][j] + hs + u * V);
+              rot_load<T, V, ALIGNED>(y[j], src + src_off[g][j] + hs + a.pairs + u * V);
+            }
+#pragma unroll
+          for (int j = 0; j < kRotTokens; ++j) {
+            if (j >= nt) break;
+            float fx[V], fy[V];
+            x[j].unpack(fx);
+            y[j].unpack(fy);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              const float2 cs = table[j * a.pairs + u * V + e];
+              const float re = fx[e], im = fy[e];
+              fx[e] = rot_re(re, im, cs);
+              fy[e] = rot_im(re, im, cs);
+            }
+            x[j].pack(fx);
+            y[j].pack(fy);
+            rot_store<T, V, ALIGNED>(x[j], dst + dst_off[g][j] + hd + u * V);
+            rot_store<T, V, ALIGNED>(y[j], dst + dst_off[g][j] + hd + a.pairs + u * V);
+          }
+        }
+      } else {  // a slot that is copied: the rest of a rotated head, or a head of v
+        const int e0 = sg.rotate ? 2 * a.pairs + (u - rot_units) * V : u * V;
+        Vec<T, V> x[kRotTokens];
+#pragma unroll
+        for (int j = 0; j < kRotTokens; ++j)
+          if (j < nt) rot_load<T, V, ALIGNED>(x[j], src + src_off[g][j] + hs + e0);
+#pragma unroll
+        for (int j = 0; j < kRotTokens; ++j)
+          if (j < nt) rot_store<T, V, ALIGNED>(x[j], dst + dst_off[g][j] + hd + e0);
+      }
+    }
+  }
+}
+
+static unsigned rot_mul(int d) { return d <= 1 ? 0u : static_cast<unsigned>((0x100000000ull + d - 1) / d); }
+
+template <typename T, int V, bool ALIGNED>
+static int rot_launch_v(RotArgs& a, bool interleaved, cudaStream_t st) {
+  const int rest = a.head_dim - 2 * a.pairs;
+  a.rot_units = interleaved ? 2 * a.pairs / V : a.pairs / V;
+  a.units = a.rot_units + rest / V;
+  a.copy_units = a.head_dim / V;
+  a.units_mul = rot_mul(a.units);
+  a.copy_mul = rot_mul(a.copy_units);
+  const long long all = static_cast<long long>(a.heads) * (a.units > a.copy_units ? a.units : a.copy_units);
+  if (all >= 65536) return ND_ERR_UNSUPPORTED;  // rot_div's range
+  const int slots = static_cast<int>(all);
+  const long long grid = (a.tokens + kRotTokens - 1) / kRotTokens;
+  if (grid > 0x7FFFFFFFLL) return ND_ERR_UNSUPPORTED;
+  const int passes = (slots + kRotThreads - 1) / kRotThreads;
+  int nt = ((slots + passes - 1) / passes + 31) / 32 * 32;
+  const void* fn;
+  if constexpr (V == 1) {  // an interleaved pair needs two elements
+    fn = (const void*)rotary_kernel<T, V, ALIGNED, false>;
+  } else {
+    fn = interleaved ? (const void*)rotary_kernel<T, V, ALIGNED, true> : (const void*)rotary_kernel<T, V, ALIGNED, false>;
+  }
+  void* params[] = {&a};
+  const size_t smem = sizeof(float2) * kRotTokens * static_cast<size_t>(a.pairs);
+  cudaError_t e = cudaLaunchKernel(fn, dim3(static_cast<unsigned>(grid)), dim3(nt), params, smem, st);
+  if (e != cudaSuccess) {
+    set_last_cuda_error(e);
+    (void)cudaGetLastError();
+    return ND_ERR_LAUNCH;
+  }
+  return ND_OK;
+}
+
+template <typename T> static int rot_launch(RotArgs& a, bool interleaved, cudaStream_t st) {
+  // the widest vector that divides every offset a slot can have and every base address: 16 bytes where R (half layout)
+  // or 2 R (interleaved) allow it; half of 72 dimensions is 36, which makes it 8 bytes for 16-bit types
+  unsigned long long mix = static_cast<unsigned long long>(a.head_dim) | (2ull * a.pairs);
+  if (!interleaved) mix |= static_cast<unsigned long long>(a.pairs);
+  unsigned long long addr = 0;
+  for (int g = 0; g < a.n_seg; ++g) {
+    const RotSeg& s = a.seg[g];
+    mix |= static_cast<unsigned long long>(s.src_h) | static_cast<unsigned long long>(s.src_s) |
+           static_cast<unsigned long long>(s.src_b) | static_cast<unsigned long long>(s.dst_h) |
+           static_cast<unsigned long long>(s.dst_s) | static_cast<unsigned long long>(s.dst_b);
+    addr |= reinterpret_cast<uintptr_t>(s.src) | reinterpret_cast<uintptr_t>(s.dst);
+  }
+  auto fits = [&](unsigned v) { return mix % v == 0 && addr % (v * sizeof(T)) == 0; };
+  if constexpr (sizeof(T) == 2) {
+    if (fits(8)) return rot_launch_v<T, 8, true>(a, interleaved, st);
+  }
+  if (fits(4)) return rot_launch_v<T, 4, true>(a, interleaved, st);
+  if (fits(2)) return rot_launch_v<T, 2, true>(a, interleaved, st);
+  // odd head dimensions, odd strides or odd addresses: single elements (adjacent pairs as two of them, where the rest
+  // of the head is even too)
+  if (!interleaved) return rot_launch_v<T, 1, true>(a, false, st);
+  if (a.head_dim % 2 == 0) return rot_launch_v<T, 2, false>(a, true, st);
+  return ND_ERR_UNSUPPORTED;
+}
+
+static int rot_entry(int dtype, RotArgs& a, int64_t batch, int64_t seq_len, int64_t heads, int64_t head_dim,
+                     const void* positions, int pos_bytes, int64_t pos_stride_b, const double* freqs, int64_t pairs,
+                     int64_t axes, int interleaved, float factor, int inverse, void* stream) {
+  a.positions = positions; a.freqs = freqs;
+  a.tokens = batch * seq_len; a.seq_len = seq_len; a.pos_b = pos_stride_b;
+  a.heads = static_cast<int>(heads); a.head_dim = static_cast<int>(head_dim);
+  a.pairs = static_cast<int>(pairs); a.axes = static_cast<int>(axes); a.pos_bytes = pos_bytes;
+  a.factor = factor; a.inverse = inverse;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  switch (dtype) {
+    case ND_F16: return rot_launch<__half>(a, interleaved != 0, st);
+    case ND_BF16: return rot_launch<__nv_bfloat16>(a, interleaved != 0, st);
+    case ND_F32: return rot_launch<float>(a, interleaved != 0, st);
+    default: return ND_ERR_UNSUPPORTED;
+  }
+}
+
+static int rot_check(int dtype, int64_t batch, int64_t seq_len, int64_t heads, int64_t head_dim, int pos_bytes,
+                     int64_t pos_stride_b, int64_t pairs, int64_t axes) {
+  if (batch < 0 || seq_len < 0 || heads <= 0 || head_dim <= 0 || pairs <= 0 || axes <= 0 || pos_stride_b < 0)
+    return ND_ERR_BAD_ARG;
+  if (pairs > head_dim / 2 || pairs % axes != 0 || (pos_bytes != 4 && pos_bytes != 8)) return ND_ERR_BAD_ARG;
+  if (dtype != ND_F16 && dtype != ND_BF16 && dtype != ND_F32) return ND_ERR_UNSUPPORTED;
+  if (pairs > kRotMaxPairs || heads > 65535 || head_dim > 65535) return ND_ERR_UNSUPPORTED;
+  if (batch > 0 && seq_len > INT64_MAX / 2 / batch) return ND_ERR_UNSUPPORTED;
+  return ND_OK;
+}
+
+}  // namespace nd
+
+extern "C" {
+
+int nd_rotary(int dtype, const void* x, void* y, int64_t batch, int64_t seq_len, int64_t heads, int64_t head_dim,
+              int64_t stride_b, int64_t stride_s, int64_t stride_h, const void* positions, int pos_bytes,
+              int64_t pos_stride_b, const double* freqs, int64_t pairs, int64_t axes, int interleaved, float factor,
+              int inverse, void* stream) {
+  using namespace nd;
+  const int rc = rot_check(dtype, batch, seq_len, heads, head_dim, pos_bytes, pos_stride_b, pairs, axes);
+  if (rc != ND_OK) return rc;
+  if (stride_b < 0 || stride_s < 0 || stride_h < 0) return ND_ERR_BAD_ARG;
+  if (batch == 0 || seq_len == 0) return ND_OK;
+  if (!x || !y || !positions || !freqs) return ND_ERR_BAD_ARG;
+  RotArgs a{};
+  a.n_seg = 1;
+  a.seg[0] = RotSeg{x, y, stride_b, stride_s, stride_h, seq_len * heads * head_dim, heads * head_dim, head_dim, 1};
+  return rot_entry(dtype, a, batch, seq_len, heads, head_dim, positions, pos_bytes, pos_stride_b, freqs, pairs, axes,
+                   interleaved, factor, inverse, stream);
+}
+
+static int qkv_rotary(bool pack, int dtype, const void* qkv, const void* const* part, int64_t batch, int64_t seq_len,
+                      int64_t heads, int64_t head_dim, const void* positions, int pos_bytes, int64_t pos_stride_b,
+                      const double* freqs, int64_t pairs, int64_t axes, int interleaved, float factor, void* stream) {
+  using namespace nd;
+  const int rc = rot_check(dtype, batch, seq_len, heads, head_dim, pos_bytes, pos_stride_b, pairs, axes);
+  if (rc != ND_OK) return rc;
+  if (batch == 0 || seq_len == 0) return ND_OK;
+  if (!qkv || !part[0] || !part[1] || !part[2] || !positions || !freqs) return ND_ERR_BAD_ARG;
+  const int64_t hidden = heads * head_dim;
+  const size_t es = dtype == ND_F32 ? 4 : 2;
+  RotArgs a{};
+  a.n_seg = 3;
+  for (int g = 0; g < 3; ++g) {
+    void* wide = const_cast<char*>(static_cast<const char*>(qkv)) + g * hidden * es;
+    void* narrow = const_cast<void*>(part[g]);
+    a.seg[g] = pack ? RotSeg{wide, narrow, seq_len * 3 * hidden, 3 * hidden, head_dim, seq_len * hidden, hidden, head_dim, g < 2}
+                    : RotSeg{narrow, wide, seq_len * hidden, hidden, head_dim, seq_len * 3 * hidden, 3 * hidden, head_dim, g < 2};
+  }
+  return rot_entry(dtype, a, batch, seq_len, heads, head_dim, positions, pos_bytes, pos_stride_b, freqs, pairs, axes,
+                   interleaved, factor, pack ? 0 : 1, stream);
+}
+
+int nd_qkv_pack_rotary_fwd(int dtype, const void* qkv, void* q, void* k, void* v, int64_t batch, int64_t seq_len,
+                           int64_t heads, int64_t head_dim, const void* positions, int pos_bytes, int64_t pos_stride_b,
+                           const double* freqs, int64_t pairs, int64_t axes, int interleaved, float factor, void* stream) {
+  const void* part[3] = {q, k, v};
+  return qkv_rotary(true, dtype, qkv, part, batch, seq_len, heads, head_dim, positions, pos_bytes, pos_stride_b, freqs,
+                    pairs, axes, interleaved, factor, stream);
+}
+
+int nd_qkv_pack_rotary_bwd(int dtype, const void* dq, const void* dk, const void* dv, void* dqkv, int64_t batch,
+                           int64_t seq_len, int64_t heads, int64_t head_dim, const void* positions, int pos_bytes,
+                           int64_t pos_stride_b, const double* freqs, int64_t pairs, int64_t axes, int interleaved,
+                           float factor, void* stream) {
+  const void* part[3] = {dq, dk, dv};
+  return qkv_rotary(false, dtype, dqkv, part, batch, seq_len, heads, head_dim, positions, pos_bytes, pos_stride_b, freqs,
+                    pairs, axes, interleaved, factor, stream);
+}
+
+}  // extern "C"

@@ -677,6 +677,100 @@ std::vector<at::Tensor> quantize_e4m3(const at::Tensor& x) {
   return {q, scale};
 }
 
+// ------------------------------------------------------------------ rotary positions
+struct RotaryTable {  // checked positions and frequencies of a [B, S, ...] tensor
+  at::Tensor positions, freqs;
+  int pos_bytes;
+  int64_t pos_stride_b, pairs, axes;
+};
+
+RotaryTable check_rotary(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& freqs, int64_t head_dim) {
+  TORCH_CHECK(dtype_id(x) >= 0, "rotary positions support fp32/fp16/bf16 tensors");
+  TORCH_CHECK(positions.is_cuda() && positions.device() == x.device(), "positions must be a CUDA tensor on x's device");
+  TORCH_CHECK(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong,
+              "positions must have dtype int32 or int64");
+  TORCH_CHECK(freqs.is_cuda() && freqs.device() == x.device(), "freqs must be a CUDA tensor on x's device");
+  TORCH_CHECK(freqs.scalar_type() == at::kDouble,
+              "freqs must have dtype float64 (in 32 bits the angles of far positions are off by whole degrees)");
+  TORCH_CHECK(freqs.dim() == 1 || freqs.dim() == 2, "freqs must have shape [R] or [axes, R]");
+  TORCH_CHECK(freqs.numel() > 0 && 2 * freqs.numel() <= head_dim, "freqs must hold 1 .. head_dim / 2 frequencies");
+  TORCH_CHECK(!freqs.requires_grad(), "freqs take no gradient: detach them");
+  RotaryTable r;
+  r.axes = freqs.dim() == 2 ? freqs.size(0) : 1;
+  r.pairs = freqs.numel();
+  const int64_t B = x.size(0), S = x.size(1), extra = freqs.dim() == 2 ? 1 : 0;
+  const bool shared = positions.dim() == 1 + extra;
+  TORCH_CHECK(shared || positions.dim() == 2 + extra, extra ? "positions must have shape [S, axes] or [B, S, axes]"
+                                                            : "positions must have shape [S] or [B, S]");
+  if (!shared) TORCH_CHECK(positions.size(0) == B, "positions batch dimension must match x");
+  TORCH_CHECK(positions.size(shared ? 0 : 1) == S, "positions sequence dimension must match x");
+  if (extra) TORCH_CHECK(positions.size(-1) == r.axes, "positions must hold one value per row of freqs");
+  r.positions = positions.contiguous();
+  r.freqs = freqs.contiguous();
+  r.pos_bytes = positions.scalar_type() == at::kLong ? 8 : 4;
+  r.pos_stride_b = shared ? 0 : S * r.axes;
+  return r;
+}
+
+// x [B, S, heads, D] (head dimensions contiguous, any other strides) -> y, contiguous; inverse: turned back
+at::Tensor fused_rotary_apply(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& freqs, bool interleaved,
+                              double factor, bool inverse) {
+  TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
+  TORCH_CHECK(x.dim() == 4, "x must have shape [B, S, heads, head_dim]");
+  c10::cuda::CUDAGuard guard(x.device());
+  const RotaryTable r = check_rotary(x, positions, freqs, x.size(3));
+  at::Tensor xc = x.stride(3) == 1 || x.numel() == 0 ? x : x.contiguous();
+  at::Tensor y = at::empty(x.sizes(), x.options());
+  if (y.numel() == 0) return y;
+  check_status(nd_rotary(dtype_id(x), xc.data_ptr(), y.data_ptr(), x.size(0), x.size(1), x.size(2), x.size(3), xc.stride(0),
+                         xc.stride(1), xc.stride(2), r.positions.data_ptr(), r.pos_bytes, r.pos_stride_b,
+                         r.freqs.data_ptr<double>(), r.pairs, r.axes, interleaved, static_cast<float>(factor), inverse,
+                         current_stream(x)),
+               "fused_rotary");
+  return y;
+}
+
+// qkv [B, S, 3 * heads * D] -> [q, k, v], q and k rotated
+std::vector<at::Tensor> fused_qkv_pack_rotary_forward(const at::Tensor& qkv, int64_t num_heads, int64_t head_dim,
+                                                      const at::Tensor& positions, const at::Tensor& freqs,
+                                                      bool interleaved, double factor) {
+  TORCH_CHECK(qkv.is_cuda(), "qkv must be a CUDA tensor");
+  TORCH_CHECK(qkv.dim() == 3 && num_heads > 0 && head_dim > 0 && qkv.size(2) == 3 * num_heads * head_dim,
+              "qkv must have shape [B, S, 3 * num_heads * head_dim]");
+  c10::cuda::CUDAGuard guard(qkv.device());
+  const RotaryTable r = check_rotary(qkv, positions, freqs, head_dim);
+  at::Tensor src = qkv.contiguous();
+  std::vector<at::Tensor> out;
+  for (int i = 0; i < 3; ++i) out.push_back(at::empty({qkv.size(0), qkv.size(1), num_heads, head_dim}, qkv.options()));
+  if (src.numel() == 0) return out;
+  check_status(nd_qkv_pack_rotary_fwd(dtype_id(qkv), src.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(),
+                                      qkv.size(0), qkv.size(1), num_heads, head_dim, r.positions.data_ptr(), r.pos_bytes,
+                                      r.pos_stride_b, r.freqs.data_ptr<double>(), r.pairs, r.axes, interleaved,
+                                      static_cast<float>(factor), current_stream(qkv)),
+               "fused_qkv_pack_rotary_forward");
+  return out;
+}
+
+at::Tensor fused_qkv_pack_rotary_backward(const at::Tensor& dq, const at::Tensor& dk, const at::Tensor& dv,
+                                          const at::Tensor& positions, const at::Tensor& freqs, bool interleaved,
+                                          double factor) {
+  TORCH_CHECK(dq.is_cuda() && dq.dim() == 4, "dq must be a CUDA tensor of shape [B, S, heads, head_dim]");
+  TORCH_CHECK(dk.sizes() == dq.sizes() && dv.sizes() == dq.sizes() && dk.scalar_type() == dq.scalar_type() &&
+                  dv.scalar_type() == dq.scalar_type() && dk.device() == dq.device() && dv.device() == dq.device(),
+              "dq, dk and dv must have one shape, dtype and device");
+  c10::cuda::CUDAGuard guard(dq.device());
+  const RotaryTable r = check_rotary(dq, positions, freqs, dq.size(3));
+  at::Tensor q = dq.contiguous(), k = dk.contiguous(), v = dv.contiguous();
+  at::Tensor dqkv = at::empty({dq.size(0), dq.size(1), 3 * dq.size(2) * dq.size(3)}, dq.options());
+  if (dqkv.numel() == 0) return dqkv;
+  check_status(nd_qkv_pack_rotary_bwd(dtype_id(dq), q.data_ptr(), k.data_ptr(), v.data_ptr(), dqkv.data_ptr(), dq.size(0),
+                                      dq.size(1), dq.size(2), dq.size(3), r.positions.data_ptr(), r.pos_bytes, r.pos_stride_b,
+                                      r.freqs.data_ptr<double>(), r.pairs, r.axes, interleaved, static_cast<float>(factor),
+                                      current_stream(dq)),
+               "fused_qkv_pack_rotary_backward");
+  return dqkv;
+}
+
 // FC1 on e4m3 operands: x_q [B, S, H], w_q [N, H] (rows [gate | value] when gated), bias (16-bit, optional),
 // scales = two device floats (x's and w's de-quantisation scales) -> y in `out_bf16 ? bf16 : fp16`
 at::Tensor fused_fc1_bias_act_forward_fp8(const at::Tensor& x_q, const at::Tensor& w_q, c10::optional<at::Tensor> bias,
@@ -729,6 +823,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fused_adaln_backward", &fused_adaln_backward, "one-pass AdaLN backward -> [dx, dscale, dshift]");
   m.def("fused_qkv_pack_forward", &fused_qkv_pack_forward, "qkv [B,S,3H] -> [q, k, v], each [B,S,heads,head_dim]");
   m.def("fused_qkv_pack_backward", &fused_qkv_pack_backward, "dq, dk, dv [B,S,heads,head_dim] -> dqkv [B,S,3H]");
+  m.def("fused_rotary_apply", &fused_rotary_apply, "rotary positions on [B,S,heads,D] (inverse: its gradient)");
+  m.def("fused_qkv_pack_rotary_forward", &fused_qkv_pack_rotary_forward, "qkv [B,S,3H] -> [q, k, v], q and k rotated");
+  m.def("fused_qkv_pack_rotary_backward", &fused_qkv_pack_rotary_backward, "dq, dk, dv -> dqkv, dq and dk turned back");
   m.def("fused_out_residual_forward", &fused_out_residual_forward, "y = x + residual (+ bias)");
   m.def("fused_geglu_forward", &fused_geglu_forward, "fused GeGLU forward (GELU-gated, tanh approx)");
   m.def("fused_geglu_backward", &fused_geglu_backward, "fused GeGLU backward");

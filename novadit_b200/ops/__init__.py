@@ -69,6 +69,13 @@ from .residual import (  # noqa: E402
     residual_adaln_ref,
     residual_adarmsnorm_ref,
 )
+from .rotary import (  # noqa: E402
+    fused_qkv_pack_rotary,
+    fused_rotary,
+    qkv_pack_rotary_ref,
+    rotary_frequencies,
+    rotary_ref,
+)
 
 __all__ = [
     "HAS_NOVADIT_CUDA",
@@ -109,4 +116,9 @@ __all__ = [
     "novadit_cuda",
     "out_residual_ref",
     "qkv_pack_ref",
+    "fused_qkv_pack_rotary",
+    "fused_rotary",
+    "qkv_pack_rotary_ref",
+    "rotary_frequencies",
+    "rotary_ref",
 ]
