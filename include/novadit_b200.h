@@ -264,6 +264,36 @@ int nd_qkv_pack_rotary_bwd(int dtype, const void* dq, const void* dk, const void
                            int64_t pos_stride_b, const double* freqs, int64_t pairs, int64_t axes, int interleaved,
                            float factor, void* stream);
 
+/* -------------------------------------------------------------------- attention to keys of another length */
+
+/* out = softmax(scale * q k^T) v per sample and head, over the keys that take part.
+ * q [batch, sq, hq, head_dim], k and v [batch, sk, hkv, head_dim] as strided views (`strides`: element strides of batch,
+ * sequence and head for q, k, v: nine values, multiples of 8; head dimensions contiguous), out contiguous like q. Query
+ * head h reads key head h / (hq / hkv). ND_F16 or ND_BF16, head_dim a multiple of 8 up to 128, bases 16-byte aligned,
+ * anything else ND_ERR_UNSUPPORTED; scale positive and finite. Which keys take part (at most one of the two): key_mask
+ * [batch, sk] bytes, non-zero = takes part; kv_lens [batch] ints, the first kv_lens[b] keys (values are clamped to
+ * 0 .. sk). Others are never looked at: they may hold NaN. A sample without keys gives zeros. Scores, sums and outputs
+ * are accumulated in fp32. `lse` (nullable; nd_attn_lse_floats values, 16-byte aligned, an order of its own) is what
+ * the backward pass needs. `ws`: nd_attn_fwd_ws_bytes bytes, 16-byte aligned, no initialisation; 0 bytes unless there
+ * is less work than SMs (then the keys are split over them and joined by a second small launch). It may be shared by
+ * launches on one stream, not by launches that may overlap. No counterpart in the reference, whose attention calls a
+ * library (novadit/modules/dit_attention.py:10-80). */
+int64_t nd_attn_lse_floats(int64_t batch, int64_t sq, int64_t hq, int64_t hkv);
+size_t nd_attn_fwd_ws_bytes(int64_t batch, int64_t sq, int64_t sk, int64_t hq, int64_t hkv, int64_t head_dim);
+int nd_attn_fwd(int dtype, const void* q, const void* k, const void* v, void* out, float* lse, const void* key_mask,
+                const int* kv_lens, int64_t batch, int64_t sq, int64_t sk, int64_t hq, int64_t hkv, int64_t head_dim,
+                const int64_t* strides, float scale, void* ws, size_t ws_bytes, void* stream);
+
+/* Gradients of nd_attn_fwd: dq, dk, dv contiguous, from dout (strided like q: `strides` holds twelve values, q, k, v,
+ * dout), the inputs, `out` (contiguous) and `lse` of the forward pass. No atomics: the same inputs give the same bits.
+ * Keys that take no part, and all keys and queries of a sample without keys, get zeros. `ws`: nd_attn_bwd_ws_bytes
+ * bytes (the row sums of dout * out; partial dk and dv where the queries are split), as above. */
+size_t nd_attn_bwd_ws_bytes(int64_t batch, int64_t sq, int64_t sk, int64_t hq, int64_t hkv, int64_t head_dim);
+int nd_attn_bwd(int dtype, const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
+                void* dq, void* dk, void* dv, const void* key_mask, const int* kv_lens, int64_t batch, int64_t sq,
+                int64_t sk, int64_t hq, int64_t hkv, int64_t head_dim, const int64_t* strides, float scale, void* ws,
+                size_t ws_bytes, void* stream);
+
 /* -------------------------------------------------------------------- FC1 */
 
 /* z = (x @ w^T) * alpha + bias, x [m,k] and w [n,k] both K-contiguous (nn.Linear layout).

@@ -42,6 +42,8 @@ CU_SOURCES = [
     "gate_act.cu",
     "rowops.cu",
     "rotary.cu",
+    "attn_fwd.cu",
+    "attn_bwd.cu",
     "quant.cu",
     "fc1.cu",
     "noalloc.cu",

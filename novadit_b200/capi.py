@@ -73,6 +73,11 @@ SIGNATURES = {
                                        c_int64, c_void_p, c_int64, c_int64, c_int, c_float, c_void_p]),
     "nd_qkv_pack_rotary_bwd": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, *[c_int64] * 4, c_void_p, c_int,
                                        c_int64, c_void_p, c_int64, c_int64, c_int, c_float, c_void_p]),
+    "nd_attn_lse_floats": (c_int64, [c_int64] * 4),
+    "nd_attn_fwd_ws_bytes": (c_size_t, [c_int64] * 6),
+    "nd_attn_fwd": (c_int, [c_int, *[c_void_p] * 7, *[c_int64] * 6, c_void_p, c_float, c_void_p, c_size_t, c_void_p]),
+    "nd_attn_bwd_ws_bytes": (c_size_t, [c_int64] * 6),
+    "nd_attn_bwd": (c_int, [c_int, *[c_void_p] * 11, *[c_int64] * 6, c_void_p, c_float, c_void_p, c_size_t, c_void_p]),
     "nd_gated_residual_fwd": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, *_SHAPE4, c_void_p]),
     "nd_gated_residual_ws_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int64]),
     "nd_adaln_fwd_residual": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,

@@ -1,0 +1,225 @@
+// What the attention kernels share: problem description, tensor maps of [B, S, heads, D] views, tcgen05 operand
+// descriptors and MMA forms, and how a sample's keys are masked.
+//
+// Rows. The queries of one key head's group are packed: a "row" is (s, g), g = 0..gp-1 the head inside a block of gp
+// query heads that share a key head (gp = the largest power of two, at most 32, that divides the group), row index
+// s * gp + g. A tile is 128 rows: one TMA box of gp heads x 128 / gp positions, so a decoding step with shared heads
+// fills a tile with all heads that read the same keys. Row statistics (log-sum-exp, delta) live in that order, each
+// head block padded to whole tiles.
+#pragma once
+
+#include "tc.cuh"
+
+namespace nd {
+
+constexpr int kTile = 128;                // rows of a query tile, keys of a key tile
+constexpr int kBlkBytes = kTile * 128;    // 64 16-bit columns of a tile, 128-byte swizzle: 16 KB
+
+struct AttnShape {
+  int batch, sq, sk, hq, hkv, d;
+  int gp, hb, rows, rows_pad, qtiles, ktiles;  // rows = sq * gp; hb = hq / gp head blocks
+  int dn;                                      // d rounded up to 16: columns of an accumulator
+};
+
+struct AttnMask {
+  const unsigned char* key_mask;  // [batch, sk], nullable
+  const int* kv_lens;             // [batch], nullable
+};
+
+inline AttnShape attn_shape(int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hkv, int64_t d) {
+  AttnShape s{};
+  s.batch = static_cast<int>(b); s.sq = static_cast<int>(sq); s.sk = static_cast<int>(sk);
+  s.hq = static_cast<int>(hq); s.hkv = static_cast<int>(hkv); s.d = static_cast<int>(d);
+  const int group = s.hq / s.hkv;
+  s.gp = 1;
+  while (s.gp < 32 && group % (2 * s.gp) == 0) s.gp *= 2;
+  s.hb = s.hq / s.gp;
+  s.rows = s.sq * s.gp;
+  s.qtiles = (s.rows + kTile - 1) / kTile;
+  s.rows_pad = s.qtiles * kTile;
+  s.ktiles = (s.sk + kTile - 1) / kTile;
+  s.dn = (s.d + 15) / 16 * 16;
+  return s;
+}
+
+int attn_launch(const void* fn, int grid, int threads, size_t smem, void** params, cudaStream_t st);
+
+inline int attn_check(int dtype, int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hkv, int64_t d, float scale) {
+  if (b < 0 || sq < 0 || sk < 0 || hq <= 0 || hkv <= 0 || d <= 0 || hq % hkv != 0) return ND_ERR_BAD_ARG;
+  if (!(scale > 0.f) || scale > 3.0e38f) return ND_ERR_BAD_ARG;
+  if (dtype != ND_F16 && dtype != ND_BF16) return ND_ERR_UNSUPPORTED;
+  if (d % 8 != 0 || d > 128) return ND_ERR_UNSUPPORTED;
+  if (b > 65535 || hq > 65535 || sq > (1 << 25) || sk > (1 << 30)) return ND_ERR_UNSUPPORTED;
+  return ND_OK;
+}
+
+// [B, S, H, D] view with element strides -> boxes of `cols` columns x `heads` heads x `pos` positions
+static bool attn_map(CUtensorMap* map, int dtype, const void* base, int64_t b, int64_t s, int64_t h, int64_t d, int64_t sb,
+                     int64_t ss, int64_t sh, int cols, int heads, int pos) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(h), static_cast<cuuint64_t>(s),
+                              static_cast<cuuint64_t>(b)};
+  // the stride of a dimension of one element is never used: any legal value
+  const cuuint64_t strides[3] = {static_cast<cuuint64_t>(h > 1 ? sh * 2 : 16), static_cast<cuuint64_t>(s > 1 ? ss * 2 : 16),
+                                 static_cast<cuuint64_t>(b > 1 ? sb * 2 : 16)};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(cols), static_cast<cuuint32_t>(heads), static_cast<cuuint32_t>(pos), 1u};
+  const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  return fn(map, dtype == ND_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+            const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// ------------------------------------------------------------------ device side
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
+}
+
+// a tile of NB 64-column blocks, `rows0` positions into the view
+template <int NB>
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int head, int pos, int b) {
+#pragma unroll
+  for (int i = 0; i < NB; ++i) tma_load_4d(dst + i * kBlkBytes, map, bar, i * 64, head, pos, b);
+}
+
+// Operand descriptors of a tile [128 rows][64-column blocks]. K-major (the columns are the reduction): 32 bytes further
+// per K = 16 step, the next block after four steps. MN-major (the rows are the reduction): 2048 bytes further per step,
+// blocks kBlkBytes apart (the leading offset).
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr, int step) {
+  return umma_desc(addr + static_cast<uint32_t>(step >> 2) * kBlkBytes + static_cast<uint32_t>(step & 3) * 32u);
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, int step) {
+  const uint32_t at = addr + static_cast<uint32_t>(step) * 2048u;
+  return (static_cast<uint64_t>((at & 0x3FFFFu) >> 4)) | (static_cast<uint64_t>(kBlkBytes >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
+}
+// M = 128, fp32 accumulator, both operands of one 16-bit type; b_mn: the B operand is MN-major
+__device__ __forceinline__ uint32_t attn_idesc(uint32_t fmt, int n, bool b_mn) {
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | (b_mn ? (1u << 16) : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
+         ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+               : "memory");
+}
+// A from tensor memory: lane = row, two 16-bit values of the reduction per column
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+               ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+               : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// S = A B^T over `steps` K = 16 steps of two K-major tiles
+__device__ __forceinline__ void issue_nt(uint32_t d, uint32_t a, uint32_t b, int steps, uint32_t idesc) {
+  for (int k = 0; k < steps; ++k) mma_ss(d, desc_k(a, k), desc_k(b, k), idesc, k != 0);
+}
+
+// Keys of sample b that take part lie below the returned index (exactly those, without a key mask). Called by whole
+// warps; every warp of a CTA gets the same answer.
+__device__ __forceinline__ int key_count(const AttnMask& m, int b, int sk, int lane) {
+  if (m.kv_lens != nullptr) {
+    const int n = __ldg(m.kv_lens + b);
+    return n < 0 ? 0 : (n > sk ? sk : n);
+  }
+  if (m.key_mask == nullptr) return sk;
+  const unsigned char* row = m.key_mask + static_cast<long long>(b) * sk;
+  int end = sk;
+  while (end > 0) {  // from the back, 1024 keys at a time: trailing padding is skipped, holes are not
+    const int base = end > 1024 ? end - 1024 : 0;
+    int last = -1;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const int at = base + i * 32 + lane;
+      if (at < end && __ldg(row + at) != 0) last = at;
+    }
+    last = __reduce_max_sync(0xffffffffu, last);
+    if (last >= 0) return last + 1;
+    end = base;
+  }
+  return 0;
+}
+
+// Which of the 128 keys of tile `kt` take part, 32 per word; called by whole warps. `partial`: some do not.
+__device__ __forceinline__ bool key_bits(const AttnMask& m, int b, int sk, int n_keys, int kt, int lane, uint32_t (&bits)[4]) {
+  bool partial = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int at = kt * kTile + i * 32;
+    const int left = n_keys - at;
+    bits[i] = left >= 32 ? 0xffffffffu : (left <= 0 ? 0u : (1u << left) - 1u);
+    if (m.key_mask != nullptr) {
+      const bool on = at + lane < n_keys && __ldg(m.key_mask + static_cast<long long>(b) * sk + at + lane) != 0;
+      bits[i] = __ballot_sync(0xffffffffu, on);
+    }
+    partial |= bits[i] != 0xffffffffu;
+  }
+  return partial;
+}
+
+// a wait of a whole warp
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, WaitSink sink, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, sink, code));
+}
+
+// zero row r of a tile: keys that do not take part may hold infinities or NaN, and 0 * NaN in a product is NaN
+template <int NB> __device__ __forceinline__ void clear_row(uint8_t* tile, int r) {
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(tile + i * kBlkBytes + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+}
+
+// One warp's 32 rows x 32 columns of 16-bit values (lane = row) through a 2 KB staging block to the copy engine.
+template <typename T>
+__device__ __forceinline__ void store_block(const CUtensorMap* map, uint8_t* stage, const float (&v)[32], int lane, int col,
+                                            int head, int pos, int b, bool inside) {
+  if (lane == 0) bulk_wait_read_all();  // the previous block has left the staging memory
+  __syncwarp();
+  const int sw = (lane >> 1) & 3;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint4 pk;
+    pk.x = pack2<T>(v[c * 8 + 0], v[c * 8 + 1]);
+    pk.y = pack2<T>(v[c * 8 + 2], v[c * 8 + 3]);
+    pk.z = pack2<T>(v[c * 8 + 4], v[c * 8 + 5]);
+    pk.w = pack2<T>(v[c * 8 + 6], v[c * 8 + 7]);
+    *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ sw) << 4)) = pk;
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0 && inside) {
+    tma_store_4d(map, stage, col, head, pos, b);
+    bulk_commit();
+  }
+}
+
+// let copies already issued land in shared memory before the CTA may exit (after an expired wait)
+__device__ __forceinline__ void settle() {
+  const unsigned long long t0 = global_ns();
+  while (global_ns() - t0 < 200000ull) __nanosleep(1000);
+}
+
+template <int COLS> __device__ __forceinline__ void tmem_alloc(uint32_t* base) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(base)), "r"(COLS) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+template <int COLS> __device__ __forceinline__ void tmem_free(uint32_t base) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(COLS) : "memory");
+}
+
+}  // namespace nd

@@ -1,0 +1,477 @@
+// Attention forward (sm_100a): out = softmax(scale q k^T) v over the keys that take part, one pass over the keys with the
+// running maximum and sum of the softmax.
+//
+// One persistent CTA per SM, 320 threads: warps 0-3 and 4-7 hold one query tile of 128 rows each (a thread owns a row),
+// warp 8 copies (TMA), warp 9 issues the MMAs. Per key tile and query tile
+//   S = Q K^T      both operands from shared memory, fp32 into 128 TMEM columns
+//   softmax        the row's 128 scores in registers; P = 2^(S c - m c) in 16 bits back over S's columns
+//   O += P V       A from tensor memory, V read where it lies (MN-major), fp32 into another 128 columns
+// Both query tiles share the key tiles; while one's softmax runs the tensor pipe works for the other.
+// The maximum is only raised when it grew by more than 2^8: P stays below 2^8 (16 bits hold that with the same relative
+// error) and O and the sum are almost never rescaled; the quotient is the same.
+// P is rounded to the element type for the second product (relative 2^-9 or 2^-12 per weight, unbiased, below the
+// rounding of the output); scores, sums and O stay in 32 bits.
+// Work items are (sample, head block, pair of query tiles, range of keys); the range is the whole length unless there
+// are fewer items than SMs: then partial (O, log-sum-exp) go through the workspace to a second small kernel.
+#include "attn.cuh"
+
+namespace nd {
+
+constexpr int kFwdThreads = 320;
+constexpr float kRaise = 8.f;  // log2 of how far the maximum may fall behind
+
+template <int NB> struct FwdCfg {
+  static constexpr int kKv = NB == 1 ? 8 : 4;  // key / value tiles in flight
+};
+
+template <int NB> struct __align__(1024) FwdSmem {
+  uint8_t q[2][NB * kBlkBytes];
+  uint8_t kv[FwdCfg<NB>::kKv][NB * kBlkBytes];
+  uint8_t out[8][2048];
+  uint64_t q_full, q_empty;
+  uint64_t kv_full[FwdCfg<NB>::kKv], kv_empty[FwdCfg<NB>::kKv];
+  uint64_t s_full[2], p_full[2], o_done[2];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+struct FwdArgs {
+  AttnShape s;
+  AttnMask mask;
+  WaitSink sink;
+  float* lse;      // [batch, hb, rows_pad], log2 of the sum of 2^(score c); nullable
+  float* part_o;   // splits > 1: [splits][batch * hb][rows_pad][d], normalised
+  float* part_l;   // splits > 1: [splits][batch * hb][rows_pad], -inf: no keys
+  float c;         // scale * log2(e)
+  int pairs, splits, tiles_per_split;
+  int items;
+};
+
+struct FwdItem {
+  int b, hb, pair, split, t0, n_t, n_keys;  // key tiles [t0, t0 + n_t)
+  bool two;                                 // the pair's second tile has rows
+};
+
+__device__ __forceinline__ FwdItem fwd_item(const FwdArgs& a, int item, int lane) {
+  FwdItem w;
+  w.split = item % a.splits;
+  int r = item / a.splits;
+  w.pair = r % a.pairs;
+  r /= a.pairs;
+  w.hb = r % a.s.hb;
+  w.b = r / a.s.hb;
+  w.two = 2 * w.pair + 1 < a.s.qtiles;
+  w.n_keys = key_count(a.mask, w.b, a.s.sk, lane);
+  const int all = (w.n_keys + kTile - 1) / kTile;
+  w.t0 = w.split * a.tiles_per_split;
+  const int left = all - w.t0;
+  w.n_t = left < 0 ? 0 : (left < a.tiles_per_split ? left : a.tiles_per_split);
+  return w;
+}
+
+template <int NB, typename T>
+__global__ void __launch_bounds__(kFwdThreads, 1)
+attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_o, const FwdArgs a) {
+  constexpr int kKv = FwdCfg<NB>::kKv;
+  constexpr int kTileBytes = NB * kBlkBytes;
+  extern __shared__ uint8_t smem_raw[];
+  FwdSmem<NB>& s = *reinterpret_cast<FwdSmem<NB>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort_flag = &s.abort_flag;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&s.q_full, 1);
+    mbar_init(&s.q_empty, 1);
+    for (int i = 0; i < kKv; ++i) {
+      mbar_init(&s.kv_full[i], 1);
+      mbar_init(&s.kv_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.p_full[i], 4);
+      mbar_init(&s.o_done[i], 1);
+    }
+    s.abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 9) tmem_alloc<512>(&s.tmem_base);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s.tmem_base;
+  griddep_launch_dependents();
+  griddep_wait();
+
+  const int group_blocks = a.s.hb / a.s.hkv;  // head blocks per key head
+  const int pos_per_tile = kTile / a.s.gp;
+  constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+
+  if (warp == 8) {
+    // ------------------------------------------------------------------ copies (one thread)
+    int it = 0, q_cnt = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; item < a.items && ok; item += gridDim.x) {
+      const FwdItem w = fwd_item(a, item, lane);
+      if (w.n_t == 0) continue;
+      if (lane == 0) {
+        const int kvh = w.hb / group_blocks;
+        ok = mbar_wait(&s.q_empty, (q_cnt & 1) ^ 1, abort_flag, a.sink, 101);
+        if (ok) {
+          mbar_expect_tx(&s.q_full, (w.two ? 2 : 1) * kTileBytes);
+          for (int t = 0; t < (w.two ? 2 : 1); ++t)
+            load_tile<NB>(s.q[t], &map_q, &s.q_full, w.hb * a.s.gp, (2 * w.pair + t) * pos_per_tile, w.b);
+        }
+        for (int j = 0; j < 2 * w.n_t && ok; ++j) {  // K(0), V(0), K(1), ...
+          const int slot = (it + j) % kKv;
+          ok = mbar_wait(&s.kv_empty[slot], (((it + j) / kKv) & 1) ^ 1, abort_flag, a.sink, 102);
+          if (!ok) break;
+          mbar_expect_tx(&s.kv_full[slot], kTileBytes);
+          load_tile<NB>(s.kv[slot], (j & 1) ? &map_v : &map_k, &s.kv_full[slot], kvh, (w.t0 + (j >> 1)) * kTile, w.b);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      it += 2 * w.n_t;
+      ++q_cnt;
+    }
+    if (!ok) settle();
+  } else if (warp == 9) {
+    // ------------------------------------------------------------------ MMA issue (one thread)
+    const int ksteps = a.s.dn / 16;
+    const uint32_t id_s = attn_idesc(kFmt, kTile, false), id_o = attn_idesc(kFmt, a.s.dn, true);
+    int it = 0, q_cnt = 0;
+    uint32_t p_cnt[2] = {0, 0};
+    bool ok = true;
+    for (int item = blockIdx.x; item < a.items && ok; item += gridDim.x) {
+      const FwdItem w = fwd_item(a, item, lane);
+      if (w.n_t == 0) continue;
+      if (lane == 0) {
+        const int nt = w.two ? 2 : 1;
+        ok = mbar_wait(&s.q_full, q_cnt & 1, abort_flag, a.sink, 103);
+        for (int j = -1; j < w.n_t && ok; ++j) {  // step j: O(j), then S(j + 1)
+          const int v_at = it + 2 * j + 1, k_at = it + 2 * j + 2;
+          const bool more = j + 1 < w.n_t;
+          if (j >= 0) ok = mbar_wait(&s.kv_full[v_at % kKv], (v_at / kKv) & 1, abort_flag, a.sink, 104);
+          for (int t = 0; t < nt && ok; ++t) {
+            if (j >= 0) {
+              ok = mbar_wait(&s.p_full[t], p_cnt[t] & 1, abort_flag, a.sink, 105);
+              if (!ok) break;
+              ++p_cnt[t];
+              tc_fence_after();
+              const uint32_t vb = smem_u32(s.kv[v_at % kKv]);
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, desc_mn(vb, k), id_o, (j > 0 || k > 0) ? 1u : 0u);
+              mma_commit(&s.o_done[t]);
+              if (t == nt - 1) mma_commit(&s.kv_empty[v_at % kKv]);
+            }
+            if (more) {
+              if (t == 0) ok = mbar_wait(&s.kv_full[k_at % kKv], (k_at / kKv) & 1, abort_flag, a.sink, 106);
+              if (!ok) break;
+              tc_fence_after();
+              issue_nt(tmem + t * 128, smem_u32(s.q[t]), smem_u32(s.kv[k_at % kKv]), ksteps, id_s);
+              mma_commit(&s.s_full[t]);
+              if (t == nt - 1) {
+                mma_commit(&s.kv_empty[k_at % kKv]);
+                if (j + 2 == w.n_t) mma_commit(&s.q_empty);  // the last scores of the item
+              }
+            }
+          }
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      it += 2 * w.n_t;
+      ++q_cnt;
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ softmax and epilogue: a thread per row
+    const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * 128;
+    uint8_t* stage = s.out[warp];
+    uint32_t s_cnt = 0, o_cnt = 0;
+    int it = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; item < a.items && ok; item += gridDim.x) {
+      const FwdItem w = fwd_item(a, item, lane);
+      const int it0 = it;
+      it += 2 * w.n_t;
+      if (t == 1 && !w.two) continue;
+      float m = -INFINITY, l = 0.f;  // maximum of the raw scores as used, sum of P
+      for (int j = 0; j < w.n_t; ++j) {
+        uint32_t bits[4];
+        const bool partial = key_bits(a.mask, w.b, a.s.sk, w.n_keys, w.t0 + j, lane, bits);
+        ok = warp_wait(&s.s_full[t], s_cnt & 1, abort_flag, a.sink, 107);
+        if (!ok) break;
+        ++s_cnt;
+        tc_fence_after();
+        float x[4][32];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tc_ld32(ts + i * 32, x[i]);
+        tc_wait_ld();
+        if (partial) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[i][e] = (bits[i] >> e) & 1u ? x[i][e] : -INFINITY;
+          if (t == 0) {  // O(j) of tile 1 is issued after that of tile 0: one warpgroup's clearing serves both
+            const int v_at = it0 + 2 * j + 1;
+            ok = warp_wait(&s.kv_full[v_at % kKv], (v_at / kKv) & 1, abort_flag, a.sink, 108);
+            if (!ok) break;
+            if (!((bits[quarter] >> lane) & 1u)) clear_row<NB>(s.kv[v_at % kKv], r);
+            fence_proxy_async_smem();
+          }
+        }
+        float mx[4] = {m, m, m, m};
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], x[i][e]);
+        const float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        const bool raise = j == 0 || !((m_new - m) * a.c <= kRaise);
+        float alpha = 1.f;
+        if (raise) {
+          alpha = m == -INFINITY ? 0.f : ex2_approx((m - m_new) * a.c);
+          m = m_new;
+          l *= alpha;
+        }
+        if (j > 0 && __any_sync(0xffffffffu, raise)) {
+          ok = warp_wait(&s.o_done[t], (o_cnt - 1) & 1, abort_flag, a.sink, 109);  // O(j - 1) is complete
+          if (!ok) break;
+          tc_fence_after();
+          for (int c = 0; c < a.s.dn; c += 16) {
+            float o[16];
+            tc_ld16(to + c, o);
+            tc_wait_ld();
+            uint32_t u[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(o[e] * alpha);
+            tc_st16(to + c, u);
+          }
+          tc_wait_st();
+        }
+        const float base = m == -INFINITY ? 0.f : m * a.c;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float p0 = ex2_approx(fmaf(x[i][e], a.c, -base)), p1 = ex2_approx(fmaf(x[i][e + 1], a.c, -base));
+            sum[i] += p0 + p1;
+            pk[e / 2] = pack2<T>(p0, p1);
+          }
+          tc_st16(ts + i * 16, pk);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.p_full[t]);
+        ++o_cnt;
+      }
+      if (!ok) break;
+      if (w.n_t > 0) {
+        ok = warp_wait(&s.o_done[t], (o_cnt - 1) & 1, abort_flag, a.sink, 110);
+        if (!ok) break;
+        tc_fence_after();
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int row = (2 * w.pair + t) * kTile + r;
+      const long long head_row = static_cast<long long>(w.b) * a.s.hb + w.hb;
+      if (a.splits > 1) {
+        const long long at = (static_cast<long long>(w.split) * a.s.batch * a.s.hb + head_row) * a.s.rows_pad + row;
+        a.part_l[at] = l == 0.f ? -INFINITY : m * a.c + log2f(l);
+        if (w.n_t > 0) {
+          for (int c = 0; c < a.s.dn; c += 16) {
+            float o[16];
+            tc_ld16(to + c, o);
+            tc_wait_ld();
+            float4* dst = reinterpret_cast<float4*>(a.part_o + at * a.s.d + c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (c + e * 4 < a.s.d && row < a.s.rows)
+                dst[e] = make_float4(o[4 * e] * inv, o[4 * e + 1] * inv, o[4 * e + 2] * inv, o[4 * e + 3] * inv);
+          }
+        }
+      } else {
+        if (a.lse != nullptr)  // +inf where there is nothing: 2^(s - inf) = 0 in the backward pass
+          a.lse[head_row * a.s.rows_pad + row] = (l == 0.f || row >= a.s.rows) ? INFINITY : m * a.c + log2f(l);
+        const int pos = (2 * w.pair + t) * pos_per_tile + quarter * 32 / a.s.gp;
+        for (int c = 0; c < a.s.d; c += 32) {
+          float o[32];
+          tc_ld32(to + c, o);
+          tc_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = l == 0.f ? 0.f : o[e] * inv;
+          store_block<T>(&map_o, stage, o, lane, c, w.hb * a.s.gp, pos, w.b, pos < a.s.sq);
+        }
+      }
+      tc_fence_before();  // these reads of O come before the next item's products
+    }
+    if (lane == 0) bulk_wait_all();  // this warp's output blocks are written before the CTA may exit
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) tmem_free<512>(tmem);
+}
+
+// Joins the key ranges of a row: weights 2^(lse_i - max), a warp per row.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_join_kernel(const FwdArgs a, T* __restrict__ out) {
+  const int lane = threadIdx.x & 31;
+  const long long rows_all = static_cast<long long>(a.s.batch) * a.s.hb * a.s.rows_pad;
+  const long long at = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  griddep_wait();
+  if (at >= rows_all) return;
+  const long long head_row = at / a.s.rows_pad;
+  const int row = static_cast<int>(at - head_row * a.s.rows_pad);
+  float top = -INFINITY;
+  for (int i = lane; i < a.splits; i += 32) top = fmaxf(top, a.part_l[i * rows_all + at]);
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  float total = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < a.splits; ++i) {
+    const float li = a.part_l[i * rows_all + at];
+    if (li == -INFINITY) continue;  // no keys: its O was never written
+    const float wgt = ex2_approx(li - top);
+    total += wgt;
+    if (lane * 4 < a.s.d && row < a.s.rows) {
+      const float4 o = *reinterpret_cast<const float4*>(a.part_o + (i * rows_all + at) * a.s.d + lane * 4);
+      acc.x = fmaf(wgt, o.x, acc.x);
+      acc.y = fmaf(wgt, o.y, acc.y);
+      acc.z = fmaf(wgt, o.z, acc.z);
+      acc.w = fmaf(wgt, o.w, acc.w);
+    }
+  }
+  if (lane == 0 && a.lse != nullptr) a.lse[at] = (total == 0.f || row >= a.s.rows) ? INFINITY : top + log2f(total);
+  if (row >= a.s.rows || lane * 4 >= a.s.d) return;
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  const int b = static_cast<int>(head_row / a.s.hb), hb = static_cast<int>(head_row - static_cast<long long>(b) * a.s.hb);
+  const int pos = row / a.s.gp, g = row - pos * a.s.gp;
+  T* dst = out + ((static_cast<long long>(b) * a.s.sq + pos) * a.s.hq + hb * a.s.gp + g) * a.s.d + lane * 4;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(acc.x * inv, acc.y * inv), pack2<T>(acc.z * inv, acc.w * inv));
+}
+
+// ------------------------------------------------------------------ host side
+static void fwd_plan(FwdArgs& a) {
+  a.pairs = (a.s.qtiles + 1) / 2;
+  const long long items = static_cast<long long>(a.s.batch) * a.s.hb * a.pairs;
+  const int sms = sm_count();
+  a.splits = 1;
+  if (items < sms && a.s.ktiles > 1) {
+    const int want = static_cast<int>(sms / items);
+    a.splits = want < a.s.ktiles ? want : a.s.ktiles;
+  }
+  a.tiles_per_split = (a.s.ktiles + a.splits - 1) / a.splits;
+  if (a.tiles_per_split < 1) a.tiles_per_split = 1;
+  a.splits = (a.s.ktiles + a.tiles_per_split - 1) / a.tiles_per_split;
+  if (a.splits < 1) a.splits = 1;
+}
+
+static size_t fwd_ws(const FwdArgs& a) {
+  if (a.splits <= 1) return 0;
+  return static_cast<size_t>(a.splits) * a.s.batch * a.s.hb * a.s.rows_pad * (a.s.d + 1) * sizeof(float);
+}
+
+int attn_launch(const void* fn, int grid, int threads, size_t smem, void** params, cudaStream_t st) {
+  if (smem > 0) {
+    const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) {
+      set_last_cuda_error(e);
+      (void)cudaGetLastError();
+      return ND_ERR_LAUNCH;
+    }
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelExC(&cfg, fn, params);
+  if (e != cudaSuccess) {
+    set_last_cuda_error(e);
+    (void)cudaGetLastError();
+    return ND_ERR_LAUNCH;
+  }
+  return ND_OK;
+}
+
+}  // namespace nd
+
+extern "C" {
+
+int64_t nd_attn_lse_floats(int64_t batch, int64_t sq, int64_t hq, int64_t hkv) {
+  if (batch <= 0 || sq <= 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || batch > 65535 || hq > 65535 || sq > (1 << 25)) return 0;
+  const nd::AttnShape s = nd::attn_shape(batch, sq, 1, hq, hkv, 8);
+  return static_cast<int64_t>(s.batch) * s.hb * s.rows_pad;
+}
+
+size_t nd_attn_fwd_ws_bytes(int64_t batch, int64_t sq, int64_t sk, int64_t hq, int64_t hkv, int64_t head_dim) {
+  if (nd::attn_check(ND_BF16, batch, sq, sk, hq, hkv, head_dim, 1.f) != ND_OK || batch == 0 || sq == 0) return 0;
+  nd::FwdArgs a{};
+  a.s = nd::attn_shape(batch, sq, sk, hq, hkv, head_dim);
+  nd::fwd_plan(a);
+  return nd::fwd_ws(a);
+}
+
+int nd_attn_fwd(int dtype, const void* q, const void* k, const void* v, void* out, float* lse, const void* key_mask,
+                const int* kv_lens, int64_t batch, int64_t sq, int64_t sk, int64_t hq, int64_t hkv, int64_t head_dim,
+                const int64_t* strides, float scale, void* ws, size_t ws_bytes, void* stream) {
+  using namespace nd;
+  const int rc = attn_check(dtype, batch, sq, sk, hq, hkv, head_dim, scale);
+  if (rc != ND_OK) return rc;
+  if (batch == 0 || sq == 0) return ND_OK;
+  if (!q || !out || !strides || (sk > 0 && (!k || !v)) || (key_mask && kv_lens)) return ND_ERR_BAD_ARG;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  FwdArgs a{};
+  a.s = attn_shape(batch, sq, sk, hq, hkv, head_dim);
+  fwd_plan(a);
+  if (static_cast<long long>(a.s.sq) * a.s.gp > (1 << 30)) return ND_ERR_UNSUPPORTED;
+  const long long items = static_cast<long long>(a.s.batch) * a.s.hb * a.pairs * a.splits;
+  if (items > INT32_MAX / 2) return ND_ERR_UNSUPPORTED;
+  if (!aligned16(q) || !aligned16(out) || (sk > 0 && (!aligned16(k) || !aligned16(v)))) return ND_ERR_UNSUPPORTED;
+  for (int i = 0; i < 9; ++i)
+    if (strides[i] < 0 || strides[i] % 8 != 0) return ND_ERR_UNSUPPORTED;
+  if (fwd_ws(a) > 0 && (ws == nullptr || ws_bytes < fwd_ws(a) || !aligned16(ws))) return ND_ERR_WORKSPACE;
+  a.items = static_cast<int>(items);
+  a.mask = AttnMask{static_cast<const unsigned char*>(key_mask), kv_lens};
+  a.sink = WaitSink{nullptr, device_error_ptr()};
+  a.lse = lse;
+  a.c = scale * 1.4426950408889634f;
+  a.part_o = static_cast<float*>(ws);
+  a.part_l = a.splits > 1 ? a.part_o + static_cast<size_t>(a.splits) * a.s.batch * a.s.hb * a.s.rows_pad * a.s.d : nullptr;
+  CUtensorMap mq, mk, mv, mo;
+  const int64_t ro = hq * head_dim;
+  const void* kb = sk > 0 ? k : q;  // never read without keys; a map needs an address
+  const void* vb = sk > 0 ? v : q;
+  const int64_t sk1 = sk > 0 ? sk : 1;
+  if (!attn_map(&mq, dtype, q, batch, sq, hq, head_dim, strides[0], strides[1], strides[2], 64, a.s.gp, kTile / a.s.gp) ||
+      !attn_map(&mk, dtype, kb, batch, sk1, hkv, head_dim, strides[3], strides[4], strides[5], 64, 1, kTile) ||
+      !attn_map(&mv, dtype, vb, batch, sk1, hkv, head_dim, strides[6], strides[7], strides[8], 64, 1, kTile) ||
+      !attn_map(&mo, dtype, out, batch, sq, hq, head_dim, sq * ro, ro, head_dim, 32, a.s.gp, 32 / a.s.gp))
+    return ND_ERR_LAUNCH;
+  const bool bf = dtype == ND_BF16, one = head_dim <= 64;
+  const void* fn = one ? (bf ? (const void*)attn_fwd_kernel<1, __nv_bfloat16> : (const void*)attn_fwd_kernel<1, __half>)
+                       : (bf ? (const void*)attn_fwd_kernel<2, __nv_bfloat16> : (const void*)attn_fwd_kernel<2, __half>);
+  const size_t smem = (one ? sizeof(FwdSmem<1>) : sizeof(FwdSmem<2>)) + 1024;
+  const int sms = sm_count();
+  void* params[] = {&mq, &mk, &mv, &mo, &a};
+  int e = attn_launch(fn, a.items < sms ? a.items : sms, kFwdThreads, smem, params, st);
+  if (e != ND_OK || a.splits == 1) return e;
+  const long long rows_all = static_cast<long long>(a.s.batch) * a.s.hb * a.s.rows_pad;
+  void* jp[] = {&a, &out};
+  return attn_launch(bf ? (const void*)attn_join_kernel<__nv_bfloat16> : (const void*)attn_join_kernel<__half>,
+                     static_cast<int>((rows_all + 7) / 8), 256, 0, jp, st);
+}
+
+}  // extern "C"

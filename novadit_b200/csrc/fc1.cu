@@ -22,14 +22,11 @@
 // Every wait on an mbarrier is bounded (1 s of %globaltimer); on expiry the waiting role raises
 // a CTA-wide abort flag, the caller's status word and the device error word are set, every role leaves its loop,
 // the producer lets its copies in flight land, and tensor memory is freed before the CTA exits.
-#include <cuda.h>
 #include <cuda_fp8.h>
 
 #include <atomic>
-#include <mutex>
 
-#include "common.cuh"
-#include "ptx.cuh"
+#include "tc.cuh"
 
 namespace nd {
 
@@ -45,20 +42,12 @@ constexpr int kStageBytes = kATileBytes + 2 * kBHalfBytes;  // 48 KB
 constexpr int kTmemCols = 512;
 constexpr int kOutBlockBytes = 32 * 32 * 2;  // 32 rows x 32 output columns of a 16-bit type
 constexpr int kGroupM = 8;       // tile rasterisation: m-blocks per group
-constexpr unsigned long long kWaitLimitNs = 1000000000ull;
-
-// Where an expired wait is recorded: the caller's status word (nullable) and the device error word that
-// nd_device_error() reads (codes 101.. there, so that they cannot be mistaken for the norm kernels' 1..3).
-struct Fc1Sink {
-  int* status;
-  int* err;
-};
 
 struct Fc1Args {
   const void* bias;        // out dtype, length n (nullable)
   void* y;
   const float* alpha_dev;  // nullable, two floats multiplied into alpha
-  Fc1Sink sink;
+  WaitSink sink;
   long long* trace;        // nullable: per-role cycle counters (see nd_tune_fc1_trace)
   float* dbias_part;       // nullable (backward only): [tiles_m * 4][n] column sums of dz per 32-row quarter
   float alpha_host;
@@ -86,27 +75,8 @@ struct __align__(1024) Fc1SmemT {
 using Fc1Smem = Fc1SmemT<kStages, 1>;
 using Fc1BwdSmem = Fc1SmemT<kBwdStages, 3>;
 
-// Bounded wait. Returns false if the CTA is aborting or the limit expired (and raises the abort).
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                          Fc1Sink sink, int code) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const unsigned long long t0 = global_ns();
-  for (uint32_t polls = 1;; ++polls) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((polls & 255u) == 0) {
-      if (*abort_flag) return false;
-      if (global_ns() - t0 > kWaitLimitNs) {
-        *abort_flag = 1;
-        if (sink.status != nullptr) atomicCAS(sink.status, 0, code);
-        if (sink.err != nullptr) atomicCAS(sink.err, 0, 100 + code);
-        return false;
-      }
-    }
-  }
-}
-
 // mbar_wait that also adds the cycles spent waiting to a per-role counter (lane 0 only; `acc` may be null)
-__device__ __forceinline__ bool mbar_wait_timed(uint64_t* bar, uint32_t parity, volatile int* abort_flag, Fc1Sink sink,
+__device__ __forceinline__ bool mbar_wait_timed(uint64_t* bar, uint32_t parity, volatile int* abort_flag, WaitSink sink,
                                                 int code, long long* acc) {
   if (acc == nullptr) return mbar_wait(bar, parity, abort_flag, sink, code);
   const long long t0 = clock64();
@@ -123,36 +93,6 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-__device__ __forceinline__ void tc_ld32(uint32_t taddr, float (&r)[32]) {
-  uint32_t* u = reinterpret_cast<uint32_t*>(r);
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
-        "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]),
-        "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]),
-        "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]),
-        "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
-      : "r"(taddr)
-      : "memory");
-}
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
-// K-major, 128B-swizzled operand tile: rows of 128 bytes, 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t umma_desc(uint32_t smem_addr) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);  // start address, 16-byte units
-  d |= static_cast<uint64_t>(1) << 16;                      // leading byte offset (unused for this layout)
-  d |= static_cast<uint64_t>(1024 >> 4) << 32;              // stride byte offset between 8-row groups
-  d |= static_cast<uint64_t>(1) << 46;                      // descriptor version of sm_100
-  d |= static_cast<uint64_t>(2) << 61;                      // SWIZZLE_128B
-  return d;
-}
-
 // dense MMA, fp32 accumulator, both operands K-major, M = 128, N = 256
 __host__ __device__ constexpr uint32_t umma_idesc(uint32_t ab_format) {
   return (1u << 4) | (ab_format << 7) | (ab_format << 10) | ((kBN >> 3) << 17) | ((kBM >> 4) << 24);
@@ -166,24 +106,6 @@ __device__ __forceinline__ void tile_coords(const Fc1Args& a, int t, int& mi, in
   const int r = t - g * per_group;
   mi = first_m + r % gm;
   ni = r / gm;
-}
-
-template <typename OUT> __device__ __forceinline__ uint32_t pack2(float a, float b);
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-  __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&v);
-}
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-  __half2 v = __floats2half2_rn(a, b);
-  return *reinterpret_cast<uint32_t*>(&v);
-}
-
-template <typename OUT> __device__ __forceinline__ float2 unpack_pair(uint32_t w);
-template <> __device__ __forceinline__ float2 unpack_pair<__nv_bfloat16>(uint32_t w) {
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-template <> __device__ __forceinline__ float2 unpack_pair<__half>(uint32_t w) {
-  return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
 // Bias of the tile's 256 accumulator columns -> one epilogue warp's shared-memory copy (fp32).
@@ -210,12 +132,6 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
                ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(src)), "r"(c0), "r"(c1)
                : "memory");
 }
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-// the issuing thread's earlier bulk stores have finished READING shared memory
-__device__ __forceinline__ void bulk_wait_read_all() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-// ... and have completed
-__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
-
 // One epilogue warp's share of a finished tile: its 32 rows (TMEM lanes at `t_lane`, first row `row0`), half of
 // the tile's column steps (`colhalf`). z = acc * alpha + bias, activation, gating, one rounding. Each step
 // yields 32 output columns per row; the warp writes them into its 2 KB staging block (row = lane, 16-byte
@@ -462,7 +378,7 @@ template <bool F8, bool PAIR, int STAGES, int STAGE_BYTES>
 __device__ __forceinline__ void mma_issue_loop(uint32_t stage0_addr, uint64_t* full, uint64_t* empty,
                                                uint64_t* tmem_full, uint64_t* tmem_empty, uint32_t tmem_base,
                                                uint32_t idesc, int my_tiles, int k_blocks, volatile int* abort_flag,
-                                               Fc1Sink sink, int code_tmem, int code_full) {
+                                               WaitSink sink, int code_tmem, int code_full) {
   const uint32_t a_lo0 = static_cast<uint32_t>(umma_desc(stage0_addr));
   const uint32_t b_lo0 = static_cast<uint32_t>(umma_desc(stage0_addr + kATileBytes));
   const uint32_t hi = static_cast<uint32_t>(umma_desc(stage0_addr) >> 32);
@@ -898,33 +814,6 @@ fc1_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant
 }
 
 // ------------------------------------------------------------------ host side
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
-  // cuTensorMapEncodeTiled is a driver call and wants a CUDA context current on the calling thread. A thread that
-  // has only used cached runtime state so far (PyTorch's autograd worker calling a backward entry point first) may
-  // have none bound yet: one runtime call that needs the context binds the device's primary context to the thread.
-  static thread_local bool context_bound = false;
-  if (!context_bound) {
-    (void)cudaFree(nullptr);
-    context_bound = true;
-  }
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-    else
-      (void)cudaGetLastError();
-  });
-  return fn;
-}
-
 // rows x k matrix, k contiguous; box = 128 bytes of k x 128 rows, 128B swizzle, zero fill out of bounds
 static bool make_map(CUtensorMap* map, CUtensorMapDataType dt, int elem_bytes, const void* base, long long rows,
                      long long k) {
@@ -1004,7 +893,7 @@ struct __align__(1024) GemmSmem {
 };
 
 struct GemmArgs {
-  Fc1Sink sink;
+  WaitSink sink;
   int m, n, k;
   int tiles_m, tiles_n, k_blocks;
 };
@@ -1242,7 +1131,7 @@ struct __align__(1024) GemmPairSmem {
 };
 
 struct GemmPairArgs {
-  Fc1Sink sink;
+  WaitSink sink;
   long long* trace;   // nullable: cycle counters of the leader's issuing thread (see nd_tune_fc1_trace)
   int* counters;      // zeroed before the launch; [boundary][rank][quarter]
   float* partials;    // [boundary][side][rank][quarter][chunk][float4 index][lane][4]
@@ -1688,7 +1577,7 @@ extern "C" int nd_fc1_fwd(int ab_dtype, int out_dtype, int act, int gated, const
   if (m > INT32_MAX - kBM || n > INT32_MAX - kBN || k > INT32_MAX - 256) return ND_ERR_UNSUPPORTED;
 
   Fc1Args a{};
-  a.bias = bias; a.y = y; a.alpha_dev = alpha_dev; a.sink = Fc1Sink{status, device_error_ptr()}; a.alpha_host = alpha_host;
+  a.bias = bias; a.y = y; a.alpha_dev = alpha_dev; a.sink = WaitSink{status, device_error_ptr()}; a.alpha_host = alpha_host;
   a.trace = g_fc1_trace.load(std::memory_order_relaxed);
   a.m = static_cast<int>(m); a.k = static_cast<int>(k); a.n = static_cast<int>(n);
   a.n_out = static_cast<int>(n_out);
@@ -1848,7 +1737,7 @@ static int fc1_bwd_dz_impl(int dtype, int act, const void* x, const void* w, con
   Fc1Args a{};
   a.dbias_part = dbias != nullptr ? static_cast<float*>(ws) : nullptr;
   a.trace = g_fc1_trace.load(std::memory_order_relaxed);
-  a.bias = bias; a.y = dz; a.sink = Fc1Sink{status, device_error_ptr()}; a.alpha_host = 1.f;
+  a.bias = bias; a.y = dz; a.sink = WaitSink{status, device_error_ptr()}; a.alpha_host = 1.f;
   a.m = static_cast<int>(m); a.k = static_cast<int>(k); a.n = static_cast<int>(n);
   a.n_out = static_cast<int>(n_out);
   a.tiles_m = static_cast<int>((m + kBM - 1) / kBM);
@@ -1975,7 +1864,7 @@ extern "C" int nd_fc1_bwd_gemm(int dtype, int op, const void* a, const void* b, 
   if (!aligned16(a) || !aligned16(b) || !aligned16(c)) return ND_ERR_UNSUPPORTED;
   if (m > INT32_MAX - kBM || n > INT32_MAX - kGemmBN || k > INT32_MAX - 256) return ND_ERR_UNSUPPORTED;
   GemmArgs g{};
-  g.sink = Fc1Sink{status, device_error_ptr()};
+  g.sink = WaitSink{status, device_error_ptr()};
   g.m = static_cast<int>(m); g.n = static_cast<int>(n); g.k = static_cast<int>(k);
   g.tiles_m = static_cast<int>((m + kBM - 1) / kBM);
   g.tiles_n = static_cast<int>((n + kGemmBN - 1) / kGemmBN);

@@ -771,6 +771,127 @@ at::Tensor fused_qkv_pack_rotary_backward(const at::Tensor& dq, const at::Tensor
   return dqkv;
 }
 
+// ------------------------------------------------------------------ attention to keys of another length
+// A [B, S, heads, D] view the copy engine can walk: contiguous head dimensions, 16-byte aligned, other strides multiples
+// of 8 elements and not zero (a broadcast dimension has no stride to walk by). Anything else is copied.
+at::Tensor attn_view(const at::Tensor& t) {
+  bool ok = (t.size(3) == 1 || t.stride(3) == 1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int i = 0; i < 3; ++i)
+    if (t.size(i) > 1) ok = ok && t.stride(i) > 0 && t.stride(i) % 8 == 0;
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+void attn_strides(const at::Tensor& t, int64_t* s) {
+  for (int i = 0; i < 3; ++i) s[i] = t.size(i) > 1 ? t.stride(i) : 8;
+}
+
+struct AttnMaskArgs {
+  at::Tensor mask, lens;  // kept alive until the launch is enqueued
+  const void* mask_p = nullptr;
+  const int* lens_p = nullptr;
+};
+
+AttnMaskArgs check_attn(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const c10::optional<at::Tensor>& key_mask,
+                        const c10::optional<at::Tensor>& kv_lens) {
+  TORCH_CHECK(q.is_cuda() && k.is_cuda() && v.is_cuda(), "q, k and v must be CUDA tensors");
+  TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "q must have shape [B, Sq, heads, D], k and v [B, Sk, kv_heads, D]");
+  TORCH_CHECK(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16, "attention supports fp16 and bf16 tensors");
+  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), "q, k and v must have one dtype");
+  TORCH_CHECK(k.device() == q.device() && v.device() == q.device(), "q, k and v must be on one device");
+  TORCH_CHECK(k.sizes() == v.sizes(), "k and v must have the same shape");
+  TORCH_CHECK(k.size(0) == q.size(0), "k and v batch dimension must match q");
+  TORCH_CHECK(k.size(3) == q.size(3), "q, k and v must have the same head dimension");
+  TORCH_CHECK(q.size(3) > 0 && q.size(3) % 8 == 0 && q.size(3) <= 128, "the head dimension must be a multiple of 8, at most 128");
+  TORCH_CHECK(q.size(2) > 0 && k.size(2) > 0 && q.size(2) % k.size(2) == 0, "the query heads must be a multiple of the key heads");
+  AttnMaskArgs m;
+  const bool has_mask = key_mask.has_value() && key_mask->defined(), has_lens = kv_lens.has_value() && kv_lens->defined();
+  TORCH_CHECK(!(has_mask && has_lens), "give key_mask or kv_lens, not both");
+  if (has_mask) {
+    TORCH_CHECK(key_mask->device() == q.device() && key_mask->scalar_type() == at::kBool, "key_mask must be a bool tensor on q's device");
+    TORCH_CHECK(key_mask->dim() == 2 && key_mask->size(0) == k.size(0) && key_mask->size(1) == k.size(1),
+                "key_mask must have shape [B, Sk]");
+    m.mask = key_mask->contiguous();
+    m.mask_p = m.mask.data_ptr();
+  }
+  if (has_lens) {
+    TORCH_CHECK(kv_lens->device() == q.device() && (kv_lens->scalar_type() == at::kInt || kv_lens->scalar_type() == at::kLong),
+                "kv_lens must be an int32 or int64 tensor on q's device");
+    TORCH_CHECK(kv_lens->dim() == 1 && kv_lens->size(0) == k.size(0), "kv_lens must have shape [B]");
+    m.lens = kv_lens->scalar_type() == at::kInt ? kv_lens->contiguous() : kv_lens->clamp(0, k.size(1)).to(at::kInt).contiguous();
+    m.lens_p = m.lens.data_ptr<int>();
+  }
+  return m;
+}
+
+at::Tensor attn_workspace(size_t bytes, const at::Tensor& like) {  // per call: no sharing across streams or captured graphs
+  return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
+}
+
+// -> [out] or, with_lse, [out, lse]
+std::vector<at::Tensor> fused_cross_attention_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                      c10::optional<at::Tensor> key_mask, c10::optional<at::Tensor> kv_lens,
+                                                      double scale, bool with_lse) {
+  TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
+  c10::cuda::CUDAGuard guard(q.device());
+  const AttnMaskArgs m = check_attn(q, k, v, key_mask, kv_lens);
+  TORCH_CHECK(static_cast<float>(scale) > 0 && scale < 3e38, "scale must be positive and finite");
+  const int64_t B = q.size(0), Sq = q.size(1), Hq = q.size(2), D = q.size(3), Sk = k.size(1), Hkv = k.size(2);
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  at::Tensor lse;
+  if (with_lse) lse = at::empty({nd_attn_lse_floats(B, Sq, Hq, Hkv)}, q.options().dtype(at::kFloat));
+  if (out.numel() > 0) {
+    at::Tensor qc = attn_view(q), kc = Sk > 0 ? attn_view(k) : k, vc = Sk > 0 ? attn_view(v) : v;
+    int64_t strides[9];
+    attn_strides(qc, strides);
+    attn_strides(kc, strides + 3);
+    attn_strides(vc, strides + 6);
+    const size_t bytes = nd_attn_fwd_ws_bytes(B, Sq, Sk, Hq, Hkv, D);
+    at::Tensor ws = attn_workspace(bytes, q);
+    check_status(nd_attn_fwd(dtype_id(q), qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), out.data_ptr(),
+                             with_lse ? lse.data_ptr<float>() : nullptr, m.mask_p, m.lens_p, B, Sq, Sk, Hq, Hkv, D, strides,
+                             static_cast<float>(scale), bytes > 0 ? ws.data_ptr() : nullptr, bytes, current_stream(q)),
+                 "fused_cross_attention_forward");
+  }
+  if (with_lse) return {out, lse};
+  return {out};
+}
+
+// -> [dq, dk, dv]
+std::vector<at::Tensor> fused_cross_attention_backward(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k,
+                                                       const at::Tensor& v, const at::Tensor& out, const at::Tensor& lse,
+                                                       c10::optional<at::Tensor> key_mask, c10::optional<at::Tensor> kv_lens,
+                                                       double scale) {
+  TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
+  c10::cuda::CUDAGuard guard(q.device());
+  const AttnMaskArgs m = check_attn(q, k, v, key_mask, kv_lens);
+  TORCH_CHECK(static_cast<float>(scale) > 0 && scale < 3e38, "scale must be positive and finite");
+  for (const at::Tensor* t : {&dout, &out})
+    TORCH_CHECK(t->sizes() == q.sizes() && t->scalar_type() == q.scalar_type() && t->device() == q.device(),
+                "dout and out must have q's shape, dtype and device");
+  const int64_t B = q.size(0), Sq = q.size(1), Hq = q.size(2), D = q.size(3), Sk = k.size(1), Hkv = k.size(2);
+  TORCH_CHECK(lse.is_cuda() && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
+                  lse.numel() == nd_attn_lse_floats(B, Sq, Hq, Hkv) && lse.device() == q.device(),
+              "lse must be the forward pass's");
+  at::Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
+  if (B == 0) return {dq, dk, dv};
+  const bool full = Sq > 0 && Sk > 0;
+  at::Tensor qc = full ? attn_view(q) : q, kc = full ? attn_view(k) : k, vc = full ? attn_view(v) : v;
+  at::Tensor gc = full ? attn_view(dout) : dout, oc = out.contiguous();
+  int64_t strides[12];
+  attn_strides(qc, strides);
+  attn_strides(kc, strides + 3);
+  attn_strides(vc, strides + 6);
+  attn_strides(gc, strides + 9);
+  const size_t bytes = nd_attn_bwd_ws_bytes(B, Sq, Sk, Hq, Hkv, D);
+  at::Tensor ws = attn_workspace(bytes, q);
+  check_status(nd_attn_bwd(dtype_id(q), gc.data_ptr(), qc.data_ptr(), kc.data_ptr(), vc.data_ptr(), oc.data_ptr(),
+                           lse.numel() > 0 ? lse.data_ptr<float>() : nullptr, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                           m.mask_p, m.lens_p, B, Sq, Sk, Hq, Hkv, D, strides, static_cast<float>(scale),
+                           bytes > 0 ? ws.data_ptr() : nullptr, bytes, current_stream(q)),
+               "fused_cross_attention_backward");
+  return {dq, dk, dv};
+}
+
 // FC1 on e4m3 operands: x_q [B, S, H], w_q [N, H] (rows [gate | value] when gated), bias (16-bit, optional),
 // scales = two device floats (x's and w's de-quantisation scales) -> y in `out_bf16 ? bf16 : fp16`
 at::Tensor fused_fc1_bias_act_forward_fp8(const at::Tensor& x_q, const at::Tensor& w_q, c10::optional<at::Tensor> bias,
@@ -823,6 +944,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fused_adaln_backward", &fused_adaln_backward, "one-pass AdaLN backward -> [dx, dscale, dshift]");
   m.def("fused_qkv_pack_forward", &fused_qkv_pack_forward, "qkv [B,S,3H] -> [q, k, v], each [B,S,heads,head_dim]");
   m.def("fused_qkv_pack_backward", &fused_qkv_pack_backward, "dq, dk, dv [B,S,heads,head_dim] -> dqkv [B,S,3H]");
+  m.def("fused_cross_attention_forward", &fused_cross_attention_forward,
+        "softmax(scale q k^T) v over the keys that take part -> [out] or [out, lse]");
+  m.def("fused_cross_attention_backward", &fused_cross_attention_backward, "its gradients -> [dq, dk, dv]");
   m.def("fused_rotary_apply", &fused_rotary_apply, "rotary positions on [B,S,heads,D] (inverse: its gradient)");
   m.def("fused_qkv_pack_rotary_forward", &fused_qkv_pack_rotary_forward, "qkv [B,S,3H] -> [q, k, v], q and k rotated");
   m.def("fused_qkv_pack_rotary_backward", &fused_qkv_pack_rotary_backward, "dq, dk, dv -> dqkv, dq and dk turned back");

@@ -69,6 +69,7 @@ from .residual import (  # noqa: E402
     residual_adaln_ref,
     residual_adarmsnorm_ref,
 )
+from .cross_attention import cross_attention_ref, fused_cross_attention  # noqa: E402
 from .rotary import (  # noqa: E402
     fused_qkv_pack_rotary,
     fused_rotary,
@@ -116,6 +117,8 @@ __all__ = [
     "novadit_cuda",
     "out_residual_ref",
     "qkv_pack_ref",
+    "cross_attention_ref",
+    "fused_cross_attention",
     "fused_qkv_pack_rotary",
     "fused_rotary",
     "qkv_pack_rotary_ref",
