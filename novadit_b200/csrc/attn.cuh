@@ -91,17 +91,27 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, 
   for (int i = 0; i < NB; ++i) tma_load_4d(dst + i * kBlkBytes, map, bar, i * 64, head, pos, b);
 }
 
-// Operand descriptors of a tile [128 rows][64-column blocks]. K-major (the columns are the reduction): 32 bytes further
-// per K = 16 step, the next block after four steps. MN-major (the rows are the reduction): 2048 bytes further per step,
-// blocks kBlkBytes apart (the leading offset).
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr, int step) {
-  return umma_desc(addr + static_cast<uint32_t>(step >> 2) * kBlkBytes + static_cast<uint32_t>(step & 3) * 32u);
+// One lane of a converged warp. The MMA warp issues under a branch on this: the compiler then knows that a single thread
+// runs it, and together with descriptors that are one addition away an MMA costs it some 10 cycles. Under a branch on the
+// thread index the same loop takes 55 cycles per MMA, with descriptors put together per MMA 110 to 150 - whatever N is,
+// where the tensor pipe needs 64 for N = 128 and 40 for N = 80 (148 CTAs of one issuing thread, K = 16, M = 128; with
+// both operands in shared memory 32 + N / 4).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
 }
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, int step) {
-  const uint32_t at = addr + static_cast<uint32_t>(step) * 2048u;
-  return (static_cast<uint64_t>((at & 0x3FFFFu) >> 4)) | (static_cast<uint64_t>(kBlkBytes >> 4) << 16) |
+
+// Operand descriptors of a tile [128 rows][64-column blocks], addresses in 16-byte units in the low word. K-major (the
+// columns are the reduction): 32 bytes further per K = 16 step, the next block after four steps. MN-major (the rows are
+// the reduction): 2048 bytes further per step, blocks kBlkBytes apart (the leading offset).
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) { return umma_desc(addr); }
+__device__ __forceinline__ constexpr uint32_t step_k(int step) { return (step >> 2) * (kBlkBytes >> 4) + (step & 3) * 2; }
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
+  return (static_cast<uint64_t>((addr & 0x3FFFFu) >> 4)) | (static_cast<uint64_t>(kBlkBytes >> 4) << 16) |
          (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
 }
+__device__ __forceinline__ constexpr uint32_t step_mn(int step) { return step * 128; }
 // M = 128, fp32 accumulator, both operands of one 16-bit type; b_mn: the B operand is MN-major
 __device__ __forceinline__ uint32_t attn_idesc(uint32_t fmt, int n, bool b_mn) {
   return (1u << 4) | (fmt << 7) | (fmt << 10) | (b_mn ? (1u << 16) : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
@@ -124,9 +134,18 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// S = A B^T over `steps` K = 16 steps of two K-major tiles
-__device__ __forceinline__ void issue_nt(uint32_t d, uint32_t a, uint32_t b, int steps, uint32_t idesc) {
-  for (int k = 0; k < steps; ++k) mma_ss(d, desc_k(a, k), desc_k(b, k), idesc, k != 0);
+// D = A B^T over `steps` K = 16 steps of two K-major tiles
+__device__ __forceinline__ void issue_nt(uint32_t d, uint64_t a, uint64_t b, int steps, uint32_t idesc) {
+  mma_ss(d, a, b, idesc, 0u);
+#pragma unroll
+  for (int k = 1; k < 8; ++k)
+    if (k < steps) mma_ss(d, a + step_k(k), b + step_k(k), idesc, 1u);
+}
+// D (+)= A B over 128 rows of B: A from tensor memory, its second half `gap` columns behind the first
+__device__ __forceinline__ void issue_tn(uint32_t d, uint32_t a, uint32_t gap, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  mma_ts(d, a, b, idesc, accumulate);
+#pragma unroll
+  for (int k = 1; k < 8; ++k) mma_ts(d, a + (k >> 2) * gap + (k & 3) * 8, b + step_mn(k), idesc, 1u);
 }
 
 // Keys of sample b that take part lie below the returned index (exactly those, without a key mask). Called by whole

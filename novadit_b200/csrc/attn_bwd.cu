@@ -137,38 +137,36 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   } else if (warp == 9) {
     const int ksteps = a.s.dn / 16;
     const uint32_t id_s = attn_idesc(kFmt, kTile, false), id_o = attn_idesc(kFmt, a.s.dn, true);
+    const uint64_t res = desc_k(smem_u32(s.res[0])), ring = desc_k(smem_u32(s.ring[0])), ring_mn = desc_mn(smem_u32(s.ring[0]));
+    constexpr uint32_t kStep = kTileBytes >> 4;
     int it = 0, cnt = 0;
-    uint32_t p_cnt = 0, ds_cnt = 0;
+    uint32_t done = 0;  // key tiles of the items before
     bool ok = true;
     for (int item = blockIdx.x; item < a.items && ok; item += gridDim.x) {
       const Item w = get(item);
       if (w.n_t == 0) continue;
-      if (lane == 0) {
+      if (elect_one()) {
         ok = mbar_wait(&s.res_full, cnt & 1, abort_flag, a.sink, 123);
         for (int j = -1; j < w.n_t && ok; ++j) {
           const int k_at = it + 2 * j, k_next = k_at + 2, v_next = k_at + 3;
           const bool more = j + 1 < w.n_t;
           // S(j + 1), once S(j) is in registers
           if (j >= 0) {
-            ok = mbar_wait(&s.p_full, p_cnt & 1, abort_flag, a.sink, 124);
+            ok = mbar_wait(&s.p_full, (done + j) & 1, abort_flag, a.sink, 124);
             if (!ok) break;
-            ++p_cnt;
           }
           if (more) {
             ok = mbar_wait(&s.full[k_next % kRing], (k_next / kRing) & 1, abort_flag, a.sink, 125);
             if (!ok) break;
             tc_fence_after();
-            issue_nt(tmem, smem_u32(s.res[0]), smem_u32(s.ring[k_next % kRing]), ksteps, id_s);
+            issue_nt(tmem, res, ring + (k_next % kRing) * kStep, ksteps, id_s);
             mma_commit(&s.s_full);
           }
           if (j >= 0) {  // dQ += dS(j) K(j)
-            ok = mbar_wait(&s.ds_full, ds_cnt & 1, abort_flag, a.sink, 126);
+            ok = mbar_wait(&s.ds_full, (done + j) & 1, abort_flag, a.sink, 126);
             if (!ok) break;
-            ++ds_cnt;
             tc_fence_after();
-            const uint32_t kb = smem_u32(s.ring[k_at % kRing]);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) mma_ts(tmem + 384, tmem + 256 + k * 8, desc_mn(kb, k), id_o, (j > 0 || k > 0) ? 1u : 0u);
+            issue_tn(tmem + 384, tmem + 256, 32, ring_mn + (k_at % kRing) * kStep, id_o, j > 0 ? 1u : 0u);
             mma_commit(&s.ds_free);
             mma_commit(&s.empty[k_at % kRing]);
             if (!more) mma_commit(&s.acc_done);
@@ -177,15 +175,16 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             ok = mbar_wait(&s.full[v_next % kRing], (v_next / kRing) & 1, abort_flag, a.sink, 127);
             if (!ok) break;
             tc_fence_after();
-            issue_nt(tmem + 128, smem_u32(s.res[1]), smem_u32(s.ring[v_next % kRing]), ksteps, id_s);
+            issue_nt(tmem + 128, res + kStep, ring + (v_next % kRing) * kStep, ksteps, id_s);
             mma_commit(&s.dp_full);
             mma_commit(&s.empty[v_next % kRing]);
             if (j + 2 == w.n_t) mma_commit(&s.res_empty);
           }
         }
       }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
+      ok = __all_sync(0xffffffffu, ok);
       it += 2 * w.n_t;
+      done += w.n_t;
       ++cnt;
     }
     __syncwarp();
@@ -395,44 +394,38 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   } else if (warp == 9) {
     const int ksteps = a.s.dn / 16;
     const uint32_t id_s = attn_idesc(kFmt, kTile, false), id_o = attn_idesc(kFmt, a.s.dn, true);
+    const uint64_t res = desc_k(smem_u32(s.res[0])), ring = desc_k(smem_u32(s.ring[0])), ring_mn = desc_mn(smem_u32(s.ring[0]));
+    constexpr uint32_t kStep = kTileBytes >> 4;
     int it = 0, cnt = 0;
-    uint32_t p_cnt = 0, ds_cnt = 0;
+    uint32_t done = 0;  // query tiles of the items before
     bool ok = true;
     for (int item = blockIdx.x; item < a.items && ok; item += gridDim.x) {
       const Item w = get(item);
       if (w.n_i == 0) continue;
-      if (lane == 0) {
+      if (elect_one()) {
         ok = mbar_wait(&s.res_full, cnt & 1, abort_flag, a.sink, 144);
         for (int i = -1; i < w.n_i && ok; ++i) {
           const int qa = it + 2 * i, da = qa + 1, qn = qa + 2, dn = qa + 3;
           const bool more = i + 1 < w.n_i;
           if (i >= 0) {  // dV += P(i) dO(i)
-            ok = mbar_wait(&s.p_full, p_cnt & 1, abort_flag, a.sink, 145);
+            ok = mbar_wait(&s.p_full, (done + i) & 1, abort_flag, a.sink, 145);
             if (!ok) break;
-            ++p_cnt;
             tc_fence_after();
-            const uint32_t db = smem_u32(s.ring[da % kRing]);
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              mma_ts(tmem + 256, tmem + (k >> 2) * 64 + (k & 3) * 8, desc_mn(db, k), id_o, (i > 0 || k > 0) ? 1u : 0u);
+            issue_tn(tmem + 256, tmem, 64, ring_mn + (da % kRing) * kStep, id_o, i > 0 ? 1u : 0u);
             mma_commit(&s.empty[da % kRing]);
           }
           if (more) {  // S(i + 1) over P(i), which dV(i) reads first
             ok = mbar_wait(&s.full[qn % kRing], (qn / kRing) & 1, abort_flag, a.sink, 146);
             if (!ok) break;
             tc_fence_after();
-            issue_nt(tmem, smem_u32(s.res[0]), smem_u32(s.ring[qn % kRing]), ksteps, id_s);
+            issue_nt(tmem, res, ring + (qn % kRing) * kStep, ksteps, id_s);
             mma_commit(&s.s_full);
           }
           if (i >= 0) {  // dK += dS(i) Q(i)
-            ok = mbar_wait(&s.ds_full, ds_cnt & 1, abort_flag, a.sink, 147);
+            ok = mbar_wait(&s.ds_full, (done + i) & 1, abort_flag, a.sink, 147);
             if (!ok) break;
-            ++ds_cnt;
             tc_fence_after();
-            const uint32_t qb = smem_u32(s.ring[qa % kRing]);
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              mma_ts(tmem + 384, tmem + 128 + (k >> 2) * 64 + (k & 3) * 8, desc_mn(qb, k), id_o, (i > 0 || k > 0) ? 1u : 0u);
+            issue_tn(tmem + 384, tmem + 128, 64, ring_mn + (qa % kRing) * kStep, id_o, i > 0 ? 1u : 0u);
             mma_commit(&s.empty[qa % kRing]);
             if (!more) mma_commit(&s.acc_done);
           }
@@ -440,14 +433,15 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             ok = mbar_wait(&s.full[dn % kRing], (dn / kRing) & 1, abort_flag, a.sink, 148);
             if (!ok) break;
             tc_fence_after();
-            issue_nt(tmem + 128, smem_u32(s.res[1]), smem_u32(s.ring[dn % kRing]), ksteps, id_s);
+            issue_nt(tmem + 128, res + kStep, ring + (dn % kRing) * kStep, ksteps, id_s);
             mma_commit(&s.dp_full);
             if (i + 2 == w.n_i) mma_commit(&s.res_empty);
           }
         }
       }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
+      ok = __all_sync(0xffffffffu, ok);
       it += 2 * w.n_i;
+      done += w.n_i;
       ++cnt;
     }
     __syncwarp();

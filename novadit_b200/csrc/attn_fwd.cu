@@ -136,32 +136,31 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     }
     if (!ok) settle();
   } else if (warp == 9) {
-    // ------------------------------------------------------------------ MMA issue (one thread)
+    // ------------------------------------------------------------------ MMA issue (one elected thread)
     const int ksteps = a.s.dn / 16;
     const uint32_t id_s = attn_idesc(kFmt, kTile, false), id_o = attn_idesc(kFmt, a.s.dn, true);
+    const uint64_t q_desc = desc_k(smem_u32(s.q[0])), k_desc = desc_k(smem_u32(s.kv[0])), v_desc = desc_mn(smem_u32(s.kv[0]));
     int it = 0, q_cnt = 0;
-    uint32_t p_cnt[2] = {0, 0};
+    uint32_t p_base[2] = {0, 0};
     bool ok = true;
     for (int item = blockIdx.x; item < a.items && ok; item += gridDim.x) {
       const FwdItem w = fwd_item(a, item, lane);
       if (w.n_t == 0) continue;
-      if (lane == 0) {
-        const int nt = w.two ? 2 : 1;
+      const int nt = w.two ? 2 : 1;
+      if (elect_one()) {
         ok = mbar_wait(&s.q_full, q_cnt & 1, abort_flag, a.sink, 103);
         for (int j = -1; j < w.n_t && ok; ++j) {  // step j: O(j), then S(j + 1)
           const int v_at = it + 2 * j + 1, k_at = it + 2 * j + 2;
           const bool more = j + 1 < w.n_t;
           if (j >= 0) ok = mbar_wait(&s.kv_full[v_at % kKv], (v_at / kKv) & 1, abort_flag, a.sink, 104);
-          for (int t = 0; t < nt && ok; ++t) {
-            if (j >= 0) {
-              ok = mbar_wait(&s.p_full[t], p_cnt[t] & 1, abort_flag, a.sink, 105);
-              if (!ok) break;
-              ++p_cnt[t];
-              tc_fence_after();
-              const uint32_t vb = smem_u32(s.kv[v_at % kKv]);
 #pragma unroll
-              for (int k = 0; k < 8; ++k)
-                mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, desc_mn(vb, k), id_o, (j > 0 || k > 0) ? 1u : 0u);
+          for (int t = 0; t < 2; ++t) {
+            if (t >= nt || !ok) break;
+            if (j >= 0) {
+              ok = mbar_wait(&s.p_full[t], (p_base[t] + j) & 1, abort_flag, a.sink, 105);
+              if (!ok) break;
+              tc_fence_after();
+              issue_tn(tmem + 256 + t * 128, tmem + t * 128, 32, v_desc + (v_at % kKv) * (kTileBytes >> 4), id_o, j > 0 ? 1u : 0u);
               mma_commit(&s.o_done[t]);
               if (t == nt - 1) mma_commit(&s.kv_empty[v_at % kKv]);
             }
@@ -169,7 +168,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
               if (t == 0) ok = mbar_wait(&s.kv_full[k_at % kKv], (k_at / kKv) & 1, abort_flag, a.sink, 106);
               if (!ok) break;
               tc_fence_after();
-              issue_nt(tmem + t * 128, smem_u32(s.q[t]), smem_u32(s.kv[k_at % kKv]), ksteps, id_s);
+              issue_nt(tmem + t * 128, q_desc + t * (kTileBytes >> 4), k_desc + (k_at % kKv) * (kTileBytes >> 4), ksteps, id_s);
               mma_commit(&s.s_full[t]);
               if (t == nt - 1) {
                 mma_commit(&s.kv_empty[k_at % kKv]);
@@ -179,8 +178,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           }
         }
       }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
+      ok = __all_sync(0xffffffffu, ok);
       it += 2 * w.n_t;
+      p_base[0] += w.n_t;
+      if (w.two) p_base[1] += w.n_t;
       ++q_cnt;
     }
     __syncwarp();
