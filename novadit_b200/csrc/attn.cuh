@@ -12,7 +12,7 @@
 
 namespace nd {
 
-constexpr int kTile = 128;                // rows of a query tile, keys of a key tile
+constexpr int kTile = 128;                // rows of a query tile; keys of a key tile in the backward pass
 constexpr int kBlkBytes = kTile * 128;    // 64 16-bit columns of a tile, 128-byte swizzle: 16 KB
 
 struct AttnShape {
@@ -84,11 +84,11 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void*
                : "memory");
 }
 
-// a tile of NB 64-column blocks, `rows0` positions into the view
-template <int NB>
+// a tile of NB 64-column blocks of ROWS rows
+template <int NB, int ROWS = kTile>
 __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int head, int pos, int b) {
 #pragma unroll
-  for (int i = 0; i < NB; ++i) tma_load_4d(dst + i * kBlkBytes, map, bar, i * 64, head, pos, b);
+  for (int i = 0; i < NB; ++i) tma_load_4d(dst + i * ROWS * 128, map, bar, i * 64, head, pos, b);
 }
 
 // One lane of a converged warp. The MMA warp issues under a branch on this: the compiler then knows that a single thread
@@ -104,11 +104,13 @@ __device__ __forceinline__ bool elect_one() {
 
 // Operand descriptors of a tile [128 rows][64-column blocks], addresses in 16-byte units in the low word. K-major (the
 // columns are the reduction): 32 bytes further per K = 16 step, the next block after four steps. MN-major (the rows are
-// the reduction): 2048 bytes further per step, blocks kBlkBytes apart (the leading offset).
+// the reduction): 2048 bytes further per step, blocks ROWS * 128 bytes apart (the leading offset).
 __device__ __forceinline__ uint64_t desc_k(uint32_t addr) { return umma_desc(addr); }
-__device__ __forceinline__ constexpr uint32_t step_k(int step) { return (step >> 2) * (kBlkBytes >> 4) + (step & 3) * 2; }
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
-  return (static_cast<uint64_t>((addr & 0x3FFFFu) >> 4)) | (static_cast<uint64_t>(kBlkBytes >> 4) << 16) |
+template <int ROWS = kTile> __device__ __forceinline__ constexpr uint32_t step_k(int step) {
+  return (step >> 2) * (ROWS * 128 >> 4) + (step & 3) * 2;
+}
+template <int ROWS = kTile> __device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
+  return (static_cast<uint64_t>((addr & 0x3FFFFu) >> 4)) | (static_cast<uint64_t>(ROWS * 128 >> 4) << 16) |
          (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) | (static_cast<uint64_t>(2) << 61);
 }
 __device__ __forceinline__ constexpr uint32_t step_mn(int step) { return step * 128; }
@@ -134,18 +136,22 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// D = A B^T over `steps` K = 16 steps of two K-major tiles
+// D = A B^T over `steps` K = 16 steps of two K-major tiles, B of ROWS rows
+template <int ROWS = kTile>
 __device__ __forceinline__ void issue_nt(uint32_t d, uint64_t a, uint64_t b, int steps, uint32_t idesc) {
   mma_ss(d, a, b, idesc, 0u);
 #pragma unroll
   for (int k = 1; k < 8; ++k)
-    if (k < steps) mma_ss(d, a + step_k(k), b + step_k(k), idesc, 1u);
+    if (k < steps) mma_ss(d, a + step_k(k), b + step_k<ROWS>(k), idesc, 1u);
 }
-// D (+)= A B over 128 rows of B: A from tensor memory, its second half `gap` columns behind the first
-__device__ __forceinline__ void issue_tn(uint32_t d, uint32_t a, uint32_t gap, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// D (+)= A B over `steps` groups of 16 rows of B: A from tensor memory, `gap` columns between its steps 3 and 4
+template <int MAX = 8>
+__device__ __forceinline__ void issue_tn(uint32_t d, uint32_t a, uint32_t gap, uint64_t b, int steps, uint32_t idesc,
+                                         uint32_t accumulate) {
   mma_ts(d, a, b, idesc, accumulate);
 #pragma unroll
-  for (int k = 1; k < 8; ++k) mma_ts(d, a + (k >> 2) * gap + (k & 3) * 8, b + step_mn(k), idesc, 1u);
+  for (int k = 1; k < MAX; ++k)
+    if (k < steps) mma_ts(d, a + (k >> 2) * gap + (k & 3) * 8, b + step_mn(k), idesc, 1u);
 }
 
 // Keys of sample b that take part lie below the returned index (exactly those, without a key mask). Called by whole
@@ -173,34 +179,56 @@ __device__ __forceinline__ int key_count(const AttnMask& m, int b, int sk, int l
   return 0;
 }
 
-// Which of the 128 keys of tile `kt` take part, 32 per word; called by whole warps. `partial`: some do not.
+// Which of the KT keys of tile `kt` take part, 32 per word; called by whole warps. True: some do not.
+template <int KT = kTile>
 __device__ __forceinline__ bool key_bits(const AttnMask& m, int b, int sk, int n_keys, int kt, int lane, uint32_t (&bits)[4]) {
   bool partial = false;
+  const int end = n_keys < (kt + 1) * KT ? n_keys : (kt + 1) * KT;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int at = kt * kTile + i * 32;
-    const int left = n_keys - at;
+    const int at = kt * KT + i * 32;
+    const int left = end - at;
+    const uint32_t all = KT - i * 32 >= 32 ? 0xffffffffu : (KT <= i * 32 ? 0u : (1u << (KT & 31)) - 1u);
     bits[i] = left >= 32 ? 0xffffffffu : (left <= 0 ? 0u : (1u << left) - 1u);
     if (m.key_mask != nullptr) {
-      const bool on = at + lane < n_keys && __ldg(m.key_mask + static_cast<long long>(b) * sk + at + lane) != 0;
+      const bool on = at + lane < end && __ldg(m.key_mask + static_cast<long long>(b) * sk + at + lane) != 0;
       bits[i] = __ballot_sync(0xffffffffu, on);
     }
-    partial |= bits[i] != 0xffffffffu;
+    partial |= bits[i] != all;
   }
   return partial;
 }
 
-// a wait of a whole warp
+// 2^y for two values on the multiply-add units instead of the special-function unit: 2^y = 2^n 2^f with n the nearest
+// integer (the rounding of y + 1.5 * 2^23 leaves it in the low bits) and a degree-4 minimax polynomial for 2^f on
+// [-1/2, 1/2] (relative error 2.7e-6 in 32 bits, fitted by a Remez exchange). y below -126 gives 2^-126, y above
+// 127 and NaN give 2^127: a sum with it shows.
+__device__ __forceinline__ float2 exp2_poly(uint64_t y2) {
+  const float2 y = f2_unpack(y2);
+  y2 = f2_pack(fmaxf(fminf(y.x, 127.f), -126.f), fmaxf(fminf(y.y, 127.f), -126.f));
+  const uint64_t t2 = f2_add(y2, f2_pack(12582912.f, 12582912.f));
+  const uint64_t f2 = f2_fma(f2_add(t2, f2_pack(-12582912.f, -12582912.f)), f2_pack(-1.f, -1.f), y2);
+  uint64_t p = f2_fma(f2_pack(0.009570102207362652f, 0.009570102207362652f), f2, f2_pack(0.05591785907745361f, 0.05591785907745361f));
+  p = f2_fma(p, f2, f2_pack(0.240247443318367f, 0.240247443318367f));
+  p = f2_fma(p, f2, f2_pack(0.6931217908859253f, 0.6931217908859253f));
+  p = f2_fma(p, f2, f2_pack(0.9999992847442627f, 0.9999992847442627f));
+  const float2 t = f2_unpack(t2), r = f2_unpack(p);
+  return make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(t.y) << 23)));
+}
+
+// a wait of a whole warp; most find the phase complete
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, WaitSink sink, int code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, sink, code));
 }
 
 // zero row r of a tile: keys that do not take part may hold infinities or NaN, and 0 * NaN in a product is NaN
-template <int NB> __device__ __forceinline__ void clear_row(uint8_t* tile, int r) {
+template <int NB, int ROWS = kTile> __device__ __forceinline__ void clear_row(uint8_t* tile, int r) {
 #pragma unroll
   for (int i = 0; i < NB; ++i)
 #pragma unroll
-    for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(tile + i * kBlkBytes + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+    for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(tile + i * ROWS * 128 + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
 }
 
 // One warp's 32 rows x 32 columns of 16-bit values (lane = row) through a 2 KB staging block to the copy engine.
@@ -232,6 +260,11 @@ __device__ __forceinline__ void settle() {
   const unsigned long long t0 = global_ns();
   while (global_ns() - t0 < 200000ull) __nanosleep(1000);
 }
+
+// Registers per thread of the calling warpgroup, given back or taken from what others gave back: over the CTA the sum must
+// not exceed what it was launched with.
+template <int N> __device__ __forceinline__ void reg_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void reg_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
 template <int COLS> __device__ __forceinline__ void tmem_alloc(uint32_t* base) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(base)), "r"(COLS) : "memory");

@@ -137,7 +137,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   } else if (warp == 9) {
     const int ksteps = a.s.dn / 16;
     const uint32_t id_s = attn_idesc(kFmt, kTile, false), id_o = attn_idesc(kFmt, a.s.dn, true);
-    const uint64_t res = desc_k(smem_u32(s.res[0])), ring = desc_k(smem_u32(s.ring[0])), ring_mn = desc_mn(smem_u32(s.ring[0]));
+    const uint64_t res = desc_k(smem_u32(s.res[0])), ring = desc_k(smem_u32(s.ring[0])), ring_mn = desc_mn<>(smem_u32(s.ring[0]));
     constexpr uint32_t kStep = kTileBytes >> 4;
     int it = 0, cnt = 0;
     uint32_t done = 0;  // key tiles of the items before
@@ -166,7 +166,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             ok = mbar_wait(&s.ds_full, (done + j) & 1, abort_flag, a.sink, 126);
             if (!ok) break;
             tc_fence_after();
-            issue_tn(tmem + 384, tmem + 256, 32, ring_mn + (k_at % kRing) * kStep, id_o, j > 0 ? 1u : 0u);
+            issue_tn(tmem + 384, tmem + 256, 32, ring_mn + (k_at % kRing) * kStep, 8, id_o, j > 0 ? 1u : 0u);
             mma_commit(&s.ds_free);
             mma_commit(&s.empty[k_at % kRing]);
             if (!more) mma_commit(&s.acc_done);
@@ -394,7 +394,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   } else if (warp == 9) {
     const int ksteps = a.s.dn / 16;
     const uint32_t id_s = attn_idesc(kFmt, kTile, false), id_o = attn_idesc(kFmt, a.s.dn, true);
-    const uint64_t res = desc_k(smem_u32(s.res[0])), ring = desc_k(smem_u32(s.ring[0])), ring_mn = desc_mn(smem_u32(s.ring[0]));
+    const uint64_t res = desc_k(smem_u32(s.res[0])), ring = desc_k(smem_u32(s.ring[0])), ring_mn = desc_mn<>(smem_u32(s.ring[0]));
     constexpr uint32_t kStep = kTileBytes >> 4;
     int it = 0, cnt = 0;
     uint32_t done = 0;  // query tiles of the items before
@@ -411,7 +411,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             ok = mbar_wait(&s.p_full, (done + i) & 1, abort_flag, a.sink, 145);
             if (!ok) break;
             tc_fence_after();
-            issue_tn(tmem + 256, tmem, 64, ring_mn + (da % kRing) * kStep, id_o, i > 0 ? 1u : 0u);
+            issue_tn(tmem + 256, tmem, 64, ring_mn + (da % kRing) * kStep, 8, id_o, i > 0 ? 1u : 0u);
             mma_commit(&s.empty[da % kRing]);
           }
           if (more) {  // S(i + 1) over P(i), which dV(i) reads first
@@ -425,7 +425,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             ok = mbar_wait(&s.ds_full, (done + i) & 1, abort_flag, a.sink, 147);
             if (!ok) break;
             tc_fence_after();
-            issue_tn(tmem + 384, tmem + 128, 64, ring_mn + (qa % kRing) * kStep, id_o, i > 0 ? 1u : 0u);
+            issue_tn(tmem + 384, tmem + 128, 64, ring_mn + (qa % kRing) * kStep, 8, id_o, i > 0 ? 1u : 0u);
             mma_commit(&s.empty[qa % kRing]);
             if (!more) mma_commit(&s.acc_done);
           }

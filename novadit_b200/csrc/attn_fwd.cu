@@ -1,14 +1,23 @@
 // Attention forward (sm_100a): out = softmax(scale q k^T) v over the keys that take part, one pass over the keys with the
 // running maximum and sum of the softmax.
 //
-// One persistent CTA per SM, 320 threads: warps 0-3 and 4-7 hold one query tile of 128 rows each (a thread owns a row),
-// warp 8 copies (TMA), warp 9 issues the MMAs. Per key tile and query tile
-//   S = Q K^T      both operands from shared memory, fp32 into 128 TMEM columns
-//   softmax        the row's 128 scores in registers; P = 2^(S c - m c) in 16 bits back over S's columns
-//   O += P V       A from tensor memory, V read where it lies (MN-major), fp32 into another 128 columns
-// Both query tiles share the key tiles; while one's softmax runs the tensor pipe works for the other.
-// The maximum is only raised when it grew by more than 2^8: P stays below 2^8 (16 bits hold that with the same relative
-// error) and O and the sum are almost never rescaled; the quotient is the same.
+// One persistent CTA per SM, 384 threads: warps 0-3 and 4-7 hold one query tile of 128 rows each (a thread owns a row),
+// warp 8 copies (TMA), warp 9 issues the MMAs (two more complete its warpgroup, which hands registers to the softmax:
+// 8 x 32 x 216 + 4 x 32 x 72 = 384 x 168, what the CTA is launched with). Per tile of KT keys and query tile
+//   S = Q K^T      both operands from shared memory, fp32 into KT TMEM columns
+//   softmax        the row's KT scores in registers; P = 2^(S c - m c) in 16 bits into KT / 2 columns
+//   O += P V       A from tensor memory, V read where it lies (MN-major), fp32 into dn columns
+// Both query tiles share the key tiles. S and P have columns of their own, so S(j + 1) is issued as soon as S(j) is in
+// registers and is there when its softmax begins: with P over S's columns the chain softmax - O - S left both warpgroups
+// waiting half of the time (4000 cycles per 128 keys and two tiles at D = 72, where the exponentials alone take 2048).
+// Tensor memory holds 512 columns, 2 (KT + KT / 2 + dn) of which are used: KT is the largest multiple of 16 that fits,
+// 128 keys for heads up to 64 dimensions, 112 up to 80, 96 up to 112, 80 for 128.
+// The maximum. Only its order of magnitude matters: any m gives the same quotient as long as nothing overflows, and
+// 16-bit floats hold a weight of 2^20 with the same relative error as one of 1. So a tile's weights are computed under the
+// maximum as it stands, chunk by chunk while the scores arrive, and their sum tells afterwards whether it was far too
+// small (then it is raised, O and the sum are rescaled and the weights computed again). Only an item's first tile and
+// tiles with masked keys look for their maximum first.
+// Two of eight pairs of exponentials go to the multiply-add units: the special-function unit gives 16 a clock.
 // P is rounded to the element type for the second product (relative 2^-9 or 2^-12 per weight, unbiased, below the
 // rounding of the output); scores, sums and O stay in 32 bits.
 // Work items are (sample, head block, pair of query tiles, range of keys); the range is the whole length unless there
@@ -17,20 +26,22 @@
 
 namespace nd {
 
-constexpr int kFwdThreads = 320;
-constexpr float kRaise = 8.f;  // log2 of how far the maximum may fall behind
+constexpr int kFwdThreads = 384;
+constexpr int kPoly = 2;       // of eight pairs of exponentials, how many go to the multiply-add units
+// Sum of a tile's weights up to which the maximum is left as it is: far from the end of the 32-bit sums, and for fp16
+// every single weight stays below 65504.
+template <typename T> constexpr float kRaise = std::is_same<T, __half>::value ? 16384.f : 1099511627776.f;
 
-template <int NB> struct FwdCfg {
+inline int fwd_key_tile(int dn) { return dn <= 64 ? 128 : (dn <= 80 ? 112 : (dn <= 112 ? 96 : 80)); }
+
+template <int NB, int KT> struct __align__(1024) FwdSmem {
   static constexpr int kKv = NB == 1 ? 8 : 4;  // key / value tiles in flight
-};
-
-template <int NB> struct __align__(1024) FwdSmem {
   uint8_t q[2][NB * kBlkBytes];
-  uint8_t kv[FwdCfg<NB>::kKv][NB * kBlkBytes];
+  uint8_t kv[kKv][NB * KT * 128];
   uint8_t out[8][2048];
   uint64_t q_full, q_empty;
-  uint64_t kv_full[FwdCfg<NB>::kKv], kv_empty[FwdCfg<NB>::kKv];
-  uint64_t s_full[2], p_full[2], o_done[2];
+  uint64_t kv_full[kKv], kv_empty[kKv];
+  uint64_t s_full[2], s_free[2], p_full[2], o_done[2];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -43,7 +54,7 @@ struct FwdArgs {
   float* part_o;   // splits > 1: [splits][batch * hb][rows_pad][d], normalised
   float* part_l;   // splits > 1: [splits][batch * hb][rows_pad], -inf: no keys
   float c;         // scale * log2(e)
-  int pairs, splits, tiles_per_split;
+  int pairs, splits, ktiles, tiles_per_split;
   int items;
 };
 
@@ -52,7 +63,7 @@ struct FwdItem {
   bool two;                                 // the pair's second tile has rows
 };
 
-__device__ __forceinline__ FwdItem fwd_item(const FwdArgs& a, int item, int lane) {
+template <int KT> __device__ __forceinline__ FwdItem fwd_item(const FwdArgs& a, int item, int lane) {
   FwdItem w;
   w.split = item % a.splits;
   int r = item / a.splits;
@@ -62,21 +73,23 @@ __device__ __forceinline__ FwdItem fwd_item(const FwdArgs& a, int item, int lane
   w.b = r / a.s.hb;
   w.two = 2 * w.pair + 1 < a.s.qtiles;
   w.n_keys = key_count(a.mask, w.b, a.s.sk, lane);
-  const int all = (w.n_keys + kTile - 1) / kTile;
+  const int all = (w.n_keys + KT - 1) / KT;
   w.t0 = w.split * a.tiles_per_split;
   const int left = all - w.t0;
   w.n_t = left < 0 ? 0 : (left < a.tiles_per_split ? left : a.tiles_per_split);
   return w;
 }
 
-template <int NB, typename T>
+template <int NB, int KT, typename T>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                 const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_o, const FwdArgs a) {
-  constexpr int kKv = FwdCfg<NB>::kKv;
-  constexpr int kTileBytes = NB * kBlkBytes;
+  using Smem = FwdSmem<NB, KT>;
+  constexpr int kKv = Smem::kKv;
+  constexpr int kQBytes = NB * kBlkBytes, kKvBytes = NB * KT * 128;
+  constexpr int kCh = KT / 16;  // chunks of 16 keys
   extern __shared__ uint8_t smem_raw[];
-  FwdSmem<NB>& s = *reinterpret_cast<FwdSmem<NB>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Smem& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &s.abort_flag;
 
@@ -89,6 +102,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.s_free[i], 4);
       mbar_init(&s.p_full[i], 4);
       mbar_init(&s.o_done[i], 1);
     }
@@ -106,19 +120,22 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const int group_blocks = a.s.hb / a.s.hkv;  // head blocks per key head
   const int pos_per_tile = kTile / a.s.gp;
   constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  const uint32_t tm_p = tmem + 2 * KT, tm_o = tmem + 3 * KT;  // S of tile t at t * KT, P at t * KT / 2, O at t * dn
 
-  if (warp == 8) {
+  if (warp >= 8) {
+   reg_give<72>();
+   if (warp == 8) {
     // ------------------------------------------------------------------ copies (one thread)
     int it = 0, q_cnt = 0;
     bool ok = true;
     for (int item = blockIdx.x; item < a.items && ok; item += gridDim.x) {
-      const FwdItem w = fwd_item(a, item, lane);
+      const FwdItem w = fwd_item<KT>(a, item, lane);
       if (w.n_t == 0) continue;
       if (lane == 0) {
         const int kvh = w.hb / group_blocks;
         ok = mbar_wait(&s.q_empty, (q_cnt & 1) ^ 1, abort_flag, a.sink, 101);
         if (ok) {
-          mbar_expect_tx(&s.q_full, (w.two ? 2 : 1) * kTileBytes);
+          mbar_expect_tx(&s.q_full, (w.two ? 2 : 1) * kQBytes);
           for (int t = 0; t < (w.two ? 2 : 1); ++t)
             load_tile<NB>(s.q[t], &map_q, &s.q_full, w.hb * a.s.gp, (2 * w.pair + t) * pos_per_tile, w.b);
         }
@@ -126,8 +143,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           const int slot = (it + j) % kKv;
           ok = mbar_wait(&s.kv_empty[slot], (((it + j) / kKv) & 1) ^ 1, abort_flag, a.sink, 102);
           if (!ok) break;
-          mbar_expect_tx(&s.kv_full[slot], kTileBytes);
-          load_tile<NB>(s.kv[slot], (j & 1) ? &map_v : &map_k, &s.kv_full[slot], kvh, (w.t0 + (j >> 1)) * kTile, w.b);
+          mbar_expect_tx(&s.kv_full[slot], kKvBytes);
+          load_tile<NB, KT>(s.kv[slot], (j & 1) ? &map_v : &map_k, &s.kv_full[slot], kvh, (w.t0 + (j >> 1)) * KT, w.b);
         }
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -135,112 +152,122 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       ++q_cnt;
     }
     if (!ok) settle();
-  } else if (warp == 9) {
+   } else if (warp == 9) {
     // ------------------------------------------------------------------ MMA issue (one elected thread)
     const int ksteps = a.s.dn / 16;
-    const uint32_t id_s = attn_idesc(kFmt, kTile, false), id_o = attn_idesc(kFmt, a.s.dn, true);
-    const uint64_t q_desc = desc_k(smem_u32(s.q[0])), k_desc = desc_k(smem_u32(s.kv[0])), v_desc = desc_mn(smem_u32(s.kv[0]));
+    const uint32_t id_o = attn_idesc(kFmt, a.s.dn, true);
+    const uint64_t q_desc = desc_k(smem_u32(s.q[0])), k_desc = desc_k(smem_u32(s.kv[0])), v_desc = desc_mn<KT>(smem_u32(s.kv[0]));
     int it = 0, q_cnt = 0;
-    uint32_t p_base[2] = {0, 0};
+    uint32_t base[2] = {0, 0};  // key tiles of the items before, per query tile
     bool ok = true;
     for (int item = blockIdx.x; item < a.items && ok; item += gridDim.x) {
-      const FwdItem w = fwd_item(a, item, lane);
+      const FwdItem w = fwd_item<KT>(a, item, lane);
       if (w.n_t == 0) continue;
       const int nt = w.two ? 2 : 1;
       if (elect_one()) {
         ok = mbar_wait(&s.q_full, q_cnt & 1, abort_flag, a.sink, 103);
-        for (int j = -1; j < w.n_t && ok; ++j) {  // step j: O(j), then S(j + 1)
-          const int v_at = it + 2 * j + 1, k_at = it + 2 * j + 2;
+        // Step j, one query tile after the other: S(j + 1), then O(j). Their softmaxes run half a step apart, and what one
+        // of them waits for must not stand behind the other's. (Polling for whichever comes first costs this thread more
+        // than the fixed order: a pass over the barriers takes it longer than an MMA group runs.)
+        for (int j = -1; j < w.n_t && ok; ++j) {
+          const int v_at = it + 2 * j + 1, k_at = v_at + 1;
+          const int s_left = w.n_keys - (w.t0 + j + 1) * KT, o_left = s_left + KT;
+          const uint32_t id_s = attn_idesc(kFmt, s_left >= KT ? KT : (s_left + 15) & ~15, false);
+          const int steps = o_left >= KT ? kCh : (o_left + 15) >> 4;
           const bool more = j + 1 < w.n_t;
-          if (j >= 0) ok = mbar_wait(&s.kv_full[v_at % kKv], (v_at / kKv) & 1, abort_flag, a.sink, 104);
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (t >= nt || !ok) break;
-            if (j >= 0) {
-              ok = mbar_wait(&s.p_full[t], (p_base[t] + j) & 1, abort_flag, a.sink, 105);
-              if (!ok) break;
-              tc_fence_after();
-              issue_tn(tmem + 256 + t * 128, tmem + t * 128, 32, v_desc + (v_at % kKv) * (kTileBytes >> 4), id_o, j > 0 ? 1u : 0u);
-              mma_commit(&s.o_done[t]);
-              if (t == nt - 1) mma_commit(&s.kv_empty[v_at % kKv]);
-            }
             if (more) {
               if (t == 0) ok = mbar_wait(&s.kv_full[k_at % kKv], (k_at / kKv) & 1, abort_flag, a.sink, 106);
+              const uint32_t n = base[t] + j + 1;  // scores of this tile so far
+              if (ok && n > 0) ok = mbar_wait(&s.s_free[t], (n - 1) & 1, abort_flag, a.sink, 104);
               if (!ok) break;
               tc_fence_after();
-              issue_nt(tmem + t * 128, q_desc + t * (kTileBytes >> 4), k_desc + (k_at % kKv) * (kTileBytes >> 4), ksteps, id_s);
+              issue_nt<KT>(tmem + t * KT, q_desc + t * (kQBytes >> 4), k_desc + (k_at % kKv) * (kKvBytes >> 4), ksteps, id_s);
               mma_commit(&s.s_full[t]);
               if (t == nt - 1) {
                 mma_commit(&s.kv_empty[k_at % kKv]);
                 if (j + 2 == w.n_t) mma_commit(&s.q_empty);  // the last scores of the item
               }
             }
+            if (j >= 0) {
+              if (t == 0) ok = mbar_wait(&s.kv_full[v_at % kKv], (v_at / kKv) & 1, abort_flag, a.sink, 113);
+              if (ok) ok = mbar_wait(&s.p_full[t], (base[t] + j) & 1, abort_flag, a.sink, 105);
+              if (!ok) break;
+              tc_fence_after();
+              issue_tn<kCh>(tm_o + t * a.s.dn, tm_p + t * (KT / 2), 32, v_desc + (v_at % kKv) * (kKvBytes >> 4), steps, id_o,
+                            j > 0 ? 1u : 0u);
+              mma_commit(&s.o_done[t]);
+              if (t == nt - 1) mma_commit(&s.kv_empty[v_at % kKv]);
+            }
           }
         }
       }
       ok = __all_sync(0xffffffffu, ok);
       it += 2 * w.n_t;
-      p_base[0] += w.n_t;
-      if (w.two) p_base[1] += w.n_t;
+      base[0] += w.n_t;
+      if (w.two) base[1] += w.n_t;
       ++q_cnt;
     }
     __syncwarp();
+   }
   } else {
+    reg_take<216>();
     // ------------------------------------------------------------------ softmax and epilogue: a thread per row
     const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * 128;
+    const uint32_t ts = tmem + lanes + t * KT, tp = tm_p + lanes + t * (KT / 2), to = tm_o + lanes + t * a.s.dn;
     uint8_t* stage = s.out[warp];
-    uint32_t s_cnt = 0, o_cnt = 0;
+    uint32_t cnt = 0;  // key tiles so far
     int it = 0;
     bool ok = true;
     for (int item = blockIdx.x; item < a.items && ok; item += gridDim.x) {
-      const FwdItem w = fwd_item(a, item, lane);
+      const FwdItem w = fwd_item<KT>(a, item, lane);
       const int it0 = it;
       it += 2 * w.n_t;
       if (t == 1 && !w.two) continue;
       float m = -INFINITY, l = 0.f;  // maximum of the raw scores as used, sum of P
-      for (int j = 0; j < w.n_t; ++j) {
-        uint32_t bits[4];
-        const bool partial = key_bits(a.mask, w.b, a.s.sk, w.n_keys, w.t0 + j, lane, bits);
-        ok = warp_wait(&s.s_full[t], s_cnt & 1, abort_flag, a.sink, 107);
-        if (!ok) break;
-        ++s_cnt;
-        tc_fence_after();
-        float x[4][32];
+      const uint64_t c2 = f2_pack(a.c, a.c);
+      float x[kCh][16];
+      uint64_t sum[2];
+      auto weights = [&](int i, uint64_t base2) {  // P of chunk i
+        uint32_t pk[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tc_ld32(ts + i * 32, x[i]);
-        tc_wait_ld();
-        if (partial) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 32; ++e) x[i][e] = (bits[i] >> e) & 1u ? x[i][e] : -INFINITY;
-          if (t == 0) {  // O(j) of tile 1 is issued after that of tile 0: one warpgroup's clearing serves both
-            const int v_at = it0 + 2 * j + 1;
-            ok = warp_wait(&s.kv_full[v_at % kKv], (v_at / kKv) & 1, abort_flag, a.sink, 108);
-            if (!ok) break;
-            if (!((bits[quarter] >> lane) & 1u)) clear_row<NB>(s.kv[v_at % kKv], r);
-            fence_proxy_async_smem();
+        for (int e = 0; e < 8; ++e) {
+          const uint64_t y = f2_fma(f2_pack(x[i][2 * e], x[i][2 * e + 1]), c2, base2);
+          float2 p;
+          if (e < kPoly) {
+            p = exp2_poly(y);
+          } else {
+            const float2 z = f2_unpack(y);
+            p = make_float2(ex2_approx(z.x), ex2_approx(z.y));
           }
+          sum[e & 1] = f2_add(sum[e & 1], f2_pack(p.x, p.y));
+          pk[e] = pack2<T>(p.x, p.y);
         }
+        tc_st8(tp + i * 8, pk);
+      };
+      auto total = [&]() {
+        const float2 v = f2_unpack(f2_add(sum[0], sum[1]));
+        return v.x + v.y;
+      };
+      auto minus_max = [&]() {
+        const float base = m == -INFINITY ? 0.f : m * a.c;
+        return f2_pack(-base, -base);
+      };
+      // raises the maximum to that of x; O follows, if there is any yet
+      auto raise_max = [&](bool have_o) {
         float mx[4] = {m, m, m, m};
 #pragma unroll
-        for (int e = 0; e < 32; ++e)
+        for (int i = 0; i < kCh; ++i)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], x[i][e]);
-        const float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        const bool raise = j == 0 || !((m_new - m) * a.c <= kRaise);
-        float alpha = 1.f;
-        if (raise) {
-          alpha = m == -INFINITY ? 0.f : ex2_approx((m - m_new) * a.c);
-          m = m_new;
-          l *= alpha;
-        }
-        if (j > 0 && __any_sync(0xffffffffu, raise)) {
-          ok = warp_wait(&s.o_done[t], (o_cnt - 1) & 1, abort_flag, a.sink, 109);  // O(j - 1) is complete
-          if (!ok) break;
-          tc_fence_after();
+          for (int e = 0; e < 16; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], x[i][e], x[i][e + 1]);
+        const float m_new = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]);
+        const float alpha = m == -INFINITY ? 0.f : ex2_approx((m - m_new) * a.c);
+        m = m_new;
+        l *= alpha;
+        if (have_o) {
           for (int c = 0; c < a.s.dn; c += 16) {
             float o[16];
             tc_ld16(to + c, o);
@@ -250,31 +277,84 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(o[e] * alpha);
             tc_st16(to + c, u);
           }
-          tc_wait_st();
         }
-        const float base = m == -INFINITY ? 0.f : m * a.c;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      };
+      for (int j = 0; j < w.n_t; ++j, ++cnt) {
+        const bool whole = a.mask.key_mask == nullptr && (w.t0 + j + 1) * KT <= w.n_keys;  // all of its keys take part
+        ok = warp_wait(&s.s_full[t], cnt & 1, abort_flag, a.sink, 107);
+        if (!ok) break;
+        tc_fence_after();
+        sum[0] = sum[1] = 0;
+        if (__builtin_expect(whole && j > 0, 1)) {
+          // Weights under the maximum as it stands, while the scores still arrive; looked at afterwards.
+          tc_ld16(ts, x[0]);
+          const uint64_t base2 = minus_max();
+          ok = warp_wait(&s.o_done[t], (cnt - 1) & 1, abort_flag, a.sink, 109);  // O(j - 1) is complete, P(j - 1) read
+          if (!ok) break;
+          tc_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float p0 = ex2_approx(fmaf(x[i][e], a.c, -base)), p1 = ex2_approx(fmaf(x[i][e + 1], a.c, -base));
-            sum[i] += p0 + p1;
-            pk[e / 2] = pack2<T>(p0, p1);
+          for (int i = 0; i < kCh; ++i) {
+            if (i + 1 < kCh) tc_ld16(ts + (i + 1) * 16, x[i + 1]);
+            weights(i, base2);
+            if (i + 1 < kCh) tc_wait_ld();
+            if (i + 2 == kCh) {  // the scores are in registers
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&s.s_free[t]);
+            }
           }
-          tc_st16(ts + i * 16, pk);
+          if (__builtin_expect(__any_sync(0xffffffffu, !(total() <= kRaise<T>)), 0)) {
+            tc_wait_st();  // the weights just written are written again
+            raise_max(true);
+            sum[0] = sum[1] = 0;
+            const uint64_t again = minus_max();
+#pragma unroll
+            for (int i = 0; i < kCh; ++i) weights(i, again);
+          }
+        } else {
+          const int left = w.n_keys - (w.t0 + j) * KT;
+          const int n_ch = left >= KT ? kCh : (left + 15) >> 4;  // the others were not even computed
+          uint32_t bits[4];
+          const bool partial = key_bits<KT>(a.mask, w.b, a.s.sk, w.n_keys, w.t0 + j, lane, bits);
+#pragma unroll
+          for (int i = 0; i < kCh; ++i) tc_ld16(ts + i * 16, x[i]);
+          tc_wait_ld();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s.s_free[t]);
+          if (partial) {
+#pragma unroll
+            for (int i = 0; i < kCh; ++i)
+#pragma unroll
+              for (int e = 0; e < 16; ++e) x[i][e] = (bits[i >> 1] >> ((i & 1) * 16 + e)) & 1u ? x[i][e] : -INFINITY;
+            if (t == 0) {  // O(j) of tile 1 is issued after that of tile 0: one warpgroup's clearing serves both
+              const int v_at = it0 + 2 * j + 1;
+              ok = warp_wait(&s.kv_full[v_at % kKv], (v_at / kKv) & 1, abort_flag, a.sink, 108);
+              if (!ok) break;
+              if (r < KT && !((bits[quarter] >> lane) & 1u)) clear_row<NB, KT>(s.kv[v_at % kKv], r);
+              fence_proxy_async_smem();
+            }
+          }
+          if (j > 0) {
+            ok = warp_wait(&s.o_done[t], (cnt - 1) & 1, abort_flag, a.sink, 111);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          raise_max(j > 0);
+          const uint64_t base2 = minus_max();
+#pragma unroll
+          for (int i = 0; i < kCh; ++i)
+            if (i < n_ch) weights(i, base2);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        l += total();
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.p_full[t]);
-        ++o_cnt;
       }
       if (!ok) break;
       if (w.n_t > 0) {
-        ok = warp_wait(&s.o_done[t], (o_cnt - 1) & 1, abort_flag, a.sink, 110);
+        ok = warp_wait(&s.o_done[t], (cnt - 1) & 1, abort_flag, a.sink, 110);
         if (!ok) break;
         tc_fence_after();
       }
@@ -301,12 +381,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           a.lse[head_row * a.s.rows_pad + row] = (l == 0.f || row >= a.s.rows) ? INFINITY : m * a.c + log2f(l);
         const int pos = (2 * w.pair + t) * pos_per_tile + quarter * 32 / a.s.gp;
         for (int c = 0; c < a.s.d; c += 32) {
-          float o[32];
-          tc_ld32(to + c, o);
+          float o[2][16];
+          tc_ld16(to + c, o[0]);
+          if (c + 16 < a.s.dn) tc_ld16(to + c + 16, o[1]);  // (columns behind dn are clipped when the block is stored)
           tc_wait_ld();
+          float v[32];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = l == 0.f ? 0.f : o[e] * inv;
-          store_block<T>(&map_o, stage, o, lane, c, w.hb * a.s.gp, pos, w.b, pos < a.s.sq);
+          for (int e = 0; e < 32; ++e) v[e] = l == 0.f ? 0.f : o[e >> 4][e & 15] * inv;
+          store_block<T>(&map_o, stage, v, lane, c, w.hb * a.s.gp, pos, w.b, pos < a.s.sq);
         }
       }
       tc_fence_before();  // these reads of O come before the next item's products
@@ -361,22 +443,33 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const FwdArgs a, T* __re
 // ------------------------------------------------------------------ host side
 static void fwd_plan(FwdArgs& a) {
   a.pairs = (a.s.qtiles + 1) / 2;
+  const int kt = fwd_key_tile(a.s.dn);
+  a.ktiles = (a.s.sk + kt - 1) / kt;
   const long long items = static_cast<long long>(a.s.batch) * a.s.hb * a.pairs;
   const int sms = sm_count();
   a.splits = 1;
-  if (items < sms && a.s.ktiles > 1) {
+  if (items < sms && a.ktiles > 1) {
     const int want = static_cast<int>(sms / items);
-    a.splits = want < a.s.ktiles ? want : a.s.ktiles;
+    a.splits = want < a.ktiles ? want : a.ktiles;
   }
-  a.tiles_per_split = (a.s.ktiles + a.splits - 1) / a.splits;
+  a.tiles_per_split = (a.ktiles + a.splits - 1) / a.splits;
   if (a.tiles_per_split < 1) a.tiles_per_split = 1;
-  a.splits = (a.s.ktiles + a.tiles_per_split - 1) / a.tiles_per_split;
+  a.splits = (a.ktiles + a.tiles_per_split - 1) / a.tiles_per_split;
   if (a.splits < 1) a.splits = 1;
 }
 
 static size_t fwd_ws(const FwdArgs& a) {
   if (a.splits <= 1) return 0;
   return static_cast<size_t>(a.splits) * a.s.batch * a.s.hb * a.s.rows_pad * (a.s.d + 1) * sizeof(float);
+}
+
+template <typename T> static const void* pick_fwd(int kt) {
+  switch (kt) {
+    case 128: return (const void*)attn_fwd_kernel<1, 128, T>;
+    case 112: return (const void*)attn_fwd_kernel<2, 112, T>;
+    case 96: return (const void*)attn_fwd_kernel<2, 96, T>;
+    default: return (const void*)attn_fwd_kernel<2, 80, T>;
+  }
 }
 
 int attn_launch(const void* fn, int grid, int threads, size_t smem, void** params, cudaStream_t st) {
@@ -456,15 +549,18 @@ int nd_attn_fwd(int dtype, const void* q, const void* k, const void* v, void* ou
   const void* kb = sk > 0 ? k : q;  // never read without keys; a map needs an address
   const void* vb = sk > 0 ? v : q;
   const int64_t sk1 = sk > 0 ? sk : 1;
+  const int kt = fwd_key_tile(a.s.dn);
   if (!attn_map(&mq, dtype, q, batch, sq, hq, head_dim, strides[0], strides[1], strides[2], 64, a.s.gp, kTile / a.s.gp) ||
-      !attn_map(&mk, dtype, kb, batch, sk1, hkv, head_dim, strides[3], strides[4], strides[5], 64, 1, kTile) ||
-      !attn_map(&mv, dtype, vb, batch, sk1, hkv, head_dim, strides[6], strides[7], strides[8], 64, 1, kTile) ||
+      !attn_map(&mk, dtype, kb, batch, sk1, hkv, head_dim, strides[3], strides[4], strides[5], 64, 1, kt) ||
+      !attn_map(&mv, dtype, vb, batch, sk1, hkv, head_dim, strides[6], strides[7], strides[8], 64, 1, kt) ||
       !attn_map(&mo, dtype, out, batch, sq, hq, head_dim, sq * ro, ro, head_dim, 32, a.s.gp, 32 / a.s.gp))
     return ND_ERR_LAUNCH;
-  const bool bf = dtype == ND_BF16, one = head_dim <= 64;
-  const void* fn = one ? (bf ? (const void*)attn_fwd_kernel<1, __nv_bfloat16> : (const void*)attn_fwd_kernel<1, __half>)
-                       : (bf ? (const void*)attn_fwd_kernel<2, __nv_bfloat16> : (const void*)attn_fwd_kernel<2, __half>);
-  const size_t smem = (one ? sizeof(FwdSmem<1>) : sizeof(FwdSmem<2>)) + 1024;
+  const bool bf = dtype == ND_BF16;
+  const void* fn = bf ? pick_fwd<__nv_bfloat16>(kt) : pick_fwd<__half>(kt);
+  const size_t smem = (kt == 128  ? sizeof(FwdSmem<1, 128>)
+                       : kt == 112 ? sizeof(FwdSmem<2, 112>)
+                       : kt == 96  ? sizeof(FwdSmem<2, 96>)
+                                   : sizeof(FwdSmem<2, 80>)) + 1024;
   const int sms = sm_count();
   void* params[] = {&mq, &mk, &mv, &mo, &a};
   int e = attn_launch(fn, a.items < sms ? a.items : sms, kFwdThreads, smem, params, st);
