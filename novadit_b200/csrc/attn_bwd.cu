@@ -6,16 +6,25 @@
 // kernel that adds dQ up in global memory, but every sum stays in tensor memory in one fixed order: no atomics, results
 // do not change from run to run, and the second operand of every product is a tile that lies in shared memory already.
 //
-// Both: one persistent CTA per SM, 320 threads, warps 0-7 the elementwise part (two warps per TMEM lane quarter, each
-// taking 64 of the tile's 128 columns), warp 8 copies, warp 9 issues the MMAs. P and dS are the A operands of the last
-// products straight from tensor memory, in 16 bits (one rounding, unbiased, below that of the output); scores, dP,
-// statistics and accumulators stay in 32 bits.
+// Both: one persistent CTA per SM, 320 threads, warps 0-3 and 4-7 the elementwise part (a thread per row, each warpgroup
+// with 64 of the tile's 128 columns), warp 8 copies, warp 9 issues the MMAs. Each half of the columns has products and
+// barriers of its own, and the issuing thread takes them half a step apart: while one warpgroup waits for its products
+// the other computes (as one group of eight warps in step, a tile of 128 x 128 took 2800 cycles for dQ and 3300 for dK and
+// dV at D = 64, where the exponentials take 1024). P and dS are the A operands of the last products straight from
+// tensor memory, in 16 bits (one rounding, unbiased, below that of the output); scores, dP, statistics and
+// accumulators stay in 32 bits.
 //
-// dQ kernel, per key tile j:  S(j) = Q K^T, dP(j) = dO V^T, dQ += dS(j) K. S(j + 1) is issued as soon as S(j) is in
-// registers, dP(j + 1) behind dQ(j).
-// dK/dV kernel, per query tile i (everything transposed: lanes are keys):  S(i) = K Q^T, dP(i) = V dO^T,
-// dV += P(i) dO, dK += dS(i) Q. P lies over S's columns and dS over dP's, each half of the columns in its own half; S(i+1)
-// is issued behind dV(i) while dS(i) is computed, dP(i + 1) behind dK(i) while the next exponentials run.
+// dQ kernel, per key tile j and half:  S(j) = Q K^T, dP(j) = dO V^T, dQ += dS(j) K. S(j + 1) is issued as soon as S(j) is
+// in registers, dP(j + 1) behind dQ(j). delta comes from the row's dO and O tiles - or, where a sample has one key tile,
+// from P and dP, exactly and without O: with few keys the rounding of O is what would be left of dS.
+// dK/dV kernel, per query tile i and half (everything transposed: lanes are keys):  S(i) = K Q^T, dP(i) = V dO^T,
+// dV += P(i) dO, dK += dS(i) Q. P lies over S's columns and dS over dP's; S(i + 1) is issued behind dV(i) while dS(i) is
+// computed, dP(i + 1) behind dK(i) while the next exponentials run. Rows of masked keys hold anything: a row of A only
+// reaches its own row of the product, and those rows are written as zeros.
+//
+// fp16. Weights below 2^-14 and gradients far from 1 would fall out of its range: P goes into its product times a power
+// of two (the length's, at most 2^12), dS times a power of two that brings the largest |dO| (of the row for dQ, of the
+// rows that share a key head for dK) to 1/16; the accumulators are scaled back.
 #include "attn.cuh"
 
 namespace nd {
@@ -26,13 +35,12 @@ struct BwdArgs {
   AttnShape s;
   AttnMask mask;
   WaitSink sink;
-  const float* lse;   // [batch, hb, rows_pad]
-  float* delta;       // [batch, hb, rows_pad]
-  const void* out;    // contiguous [B, Sq, Hq, D]
-  const void* dout;   // strided
-  long long do_b, do_s, do_h;
+  const float* lse;   // [batch, hb, rows_pad]: minus the log-sum-exp
+  float* delta;       // [batch, hb, rows_pad]: minus delta
+  float* peak;        // fp16: [batch, hb, rows_pad], largest |dO| of a row
   float* part;        // dK/dV, splits > 1: [splits][2][B * Sk * Hkv][D]
   float c, scale;
+  float p_shift;      // fp16, dK/dV: log2 of the factor on P
   int items;
   int splits, steps, steps_per_split;  // dK/dV: query tiles of all head blocks of a key head
 };
@@ -45,9 +53,13 @@ template <int NB> struct __align__(1024) BwdSmem {
   alignas(16) float stat[kRing / 2][2][kTile];  // dK/dV: log-sum-exp and delta of the query tile
   uint64_t res_full, res_empty;
   uint64_t full[kRing], empty[kRing];
-  uint64_t s_full, dp_full;   // MMA -> elementwise
-  uint64_t p_full, ds_full;   // elementwise -> MMA (dQ: p_full = "S is in registers")
-  uint64_t ds_free, acc_done; // dQ: dS has been read; both: the accumulators are complete
+  uint64_t s_full[2], dp_full[2];   // MMA -> elementwise, per half
+  uint64_t p_full[2], ds_full[2];   // elementwise -> MMA (dQ: p_full = "S is in registers")
+  uint64_t ds_free[2];              // dQ: dS has been read
+  uint64_t acc_done;                // the accumulators are complete
+  uint64_t o_read;                  // dQ: the elementwise warps have read dO and O
+  uint64_t pair[4];                 // dQ: both halves of 32 rows have written to `red`
+  float red[2][2][kTile];           // dQ: [exchange parity][half][row]
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -59,25 +71,48 @@ template <int NB> __device__ __forceinline__ void bwd_init(BwdSmem<NB>& s) {
     mbar_init(&s.full[i], 1);
     mbar_init(&s.empty[i], 1);
   }
-  mbar_init(&s.s_full, 1);
-  mbar_init(&s.dp_full, 1);
-  mbar_init(&s.p_full, 8);
-  mbar_init(&s.ds_full, 8);
-  mbar_init(&s.ds_free, 1);
+  for (int h = 0; h < 2; ++h) {
+    mbar_init(&s.s_full[h], 1);
+    mbar_init(&s.dp_full[h], 1);
+    mbar_init(&s.p_full[h], 4);
+    mbar_init(&s.ds_full[h], 4);
+    mbar_init(&s.ds_free[h], 1);
+  }
+  for (int i = 0; i < 4; ++i) mbar_init(&s.pair[i], 2);
   mbar_init(&s.acc_done, 1);
+  mbar_init(&s.o_read, 8);
   s.abort_flag = 0;
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }
 
+// fp16: the power of two that brings `peak` to 2^-4 (1 where there is nothing to scale)
+__device__ __forceinline__ float grad_factor(float peak) {
+  if (!(peak > 0.f) || isinf(peak)) return 1.f;
+  const int e = static_cast<int>((__float_as_uint(peak) >> 23) & 255u) - 127;  // peak is a 16-bit value: a normal number
+  return __uint_as_float(static_cast<uint32_t>(127 - 4 - e) << 23);
+}
+
+// largest |value| of four 16-bit pairs
+template <typename T> __device__ __forceinline__ float peak8(const uint4& v, float top) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 f = unpack_pair<T>(w[e]);
+    top = max3(top, fabsf(f.x), fabsf(f.y));
+  }
+  return top;
+}
+
 // ------------------------------------------------------------------ dQ
-// TMEM columns: S 0, dP 128, dS 256 (64 columns of 16-bit pairs), dQ 384
+// TMEM columns: S 0, dP 128, dS 256 (32 columns of 16-bit pairs per half), dQ 384
 template <int NB, typename T>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
-               const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-               const __grid_constant__ CUtensorMap map_dq, const BwdArgs a) {
+               const __grid_constant__ CUtensorMap map_o, const __grid_constant__ CUtensorMap map_k,
+               const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_dq, const BwdArgs a) {
   constexpr int kRing = BwdSmem<NB>::kRing;
   constexpr int kTileBytes = NB * kBlkBytes;
+  constexpr bool kHalf = std::is_same<T, __half>::value;
   extern __shared__ uint8_t smem_raw[];
   BwdSmem<NB>& s = *reinterpret_cast<BwdSmem<NB>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -96,6 +131,8 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   struct Item {
     int b, hb, qt, n_keys, n_t;
+    int o;      // 1: an O tile comes first in the ring
+    int n1;     // key tiles of the second half (the last one may have no keys there)
   };
   auto get = [&](int item) {
     Item w;
@@ -105,6 +142,8 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     w.b = r / a.s.hb;
     w.n_keys = key_count(a.mask, w.b, a.s.sk, lane);
     w.n_t = (w.n_keys + kTile - 1) / kTile;
+    w.n1 = (w.n_keys + 63) / kTile;
+    w.o = w.n_t > 1 ? 1 : 0;
     return w;
   };
 
@@ -121,70 +160,120 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           load_tile<NB>(s.res[0], &map_q, &s.res_full, w.hb * a.s.gp, w.qt * pos_per_tile, w.b);
           load_tile<NB>(s.res[1], &map_do, &s.res_full, w.hb * a.s.gp, w.qt * pos_per_tile, w.b);
         }
-        for (int j = 0; j < 2 * w.n_t && ok; ++j) {
-          const int slot = (it + j) % kRing;
-          ok = mbar_wait(&s.empty[slot], (((it + j) / kRing) & 1) ^ 1, abort_flag, a.sink, 122);
+        for (int j = -w.o; j < 2 * w.n_t && ok; ++j) {  // (O,) K(0), V(0), K(1), ...
+          const int at = it + w.o + j, slot = at % kRing;
+          ok = mbar_wait(&s.empty[slot], ((at / kRing) & 1) ^ 1, abort_flag, a.sink, 122);
           if (!ok) break;
           mbar_expect_tx(&s.full[slot], kTileBytes);
-          load_tile<NB>(s.ring[slot], (j & 1) ? &map_v : &map_k, &s.full[slot], w.hb / group_blocks, (j >> 1) * kTile, w.b);
+          if (j < 0) load_tile<NB>(s.ring[slot], &map_o, &s.full[slot], w.hb * a.s.gp, w.qt * pos_per_tile, w.b);
+          else load_tile<NB>(s.ring[slot], (j & 1) ? &map_v : &map_k, &s.full[slot], w.hb / group_blocks, (j >> 1) * kTile, w.b);
         }
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
-      it += 2 * w.n_t;
+      it += w.o + 2 * w.n_t;
       ++cnt;
     }
     if (!ok) settle();
   } else if (warp == 9) {
     const int ksteps = a.s.dn / 16;
-    const uint32_t id_s = attn_idesc(kFmt, kTile, false), id_o = attn_idesc(kFmt, a.s.dn, true);
+    const uint32_t id_o = attn_idesc(kFmt, a.s.dn, true);
     const uint64_t res = desc_k(smem_u32(s.res[0])), ring = desc_k(smem_u32(s.ring[0])), ring_mn = desc_mn<>(smem_u32(s.ring[0]));
     constexpr uint32_t kStep = kTileBytes >> 4;
-    int it = 0, cnt = 0;
-    uint32_t done = 0;  // key tiles of the items before
+    constexpr uint32_t kHalfRows = 64 * 128 >> 4;  // the second half of a tile's rows
+    int it = 0, cnt = 0, o_cnt = 0;
+    uint32_t done[2] = {0, 0};  // key tiles of the items before, per half
     bool ok = true;
     for (int item = blockIdx.x; item < a.items && ok; item += gridDim.x) {
       const Item w = get(item);
       if (w.n_t == 0) continue;
       if (elect_one()) {
-        ok = mbar_wait(&s.res_full, cnt & 1, abort_flag, a.sink, 123);
-        for (int j = -1; j < w.n_t && ok; ++j) {
-          const int k_at = it + 2 * j, k_next = k_at + 2, v_next = k_at + 3;
-          const bool more = j + 1 < w.n_t;
-          // S(j + 1), once S(j) is in registers
-          if (j >= 0) {
-            ok = mbar_wait(&s.p_full, (done + j) & 1, abort_flag, a.sink, 124);
+        const int n_h[2] = {w.n_t, w.n1};
+        const int it1 = it + w.o;
+        auto keys = [&](int j, int h) {  // of this half, in 16s
+          const int left = w.n_keys - j * kTile - h * 64;
+          return left >= 64 ? 64 : (left + 15) & ~15;
+        };
+        auto wait = [&](uint64_t* bar, uint32_t n, int code) {
+          if (ok) ok = mbar_wait(bar, n & 1, abort_flag, a.sink, code);
+          return ok;
+        };
+        auto full = [&](int at, int code) { return wait(&s.full[at % kRing], static_cast<uint32_t>(at / kRing), code); };
+        auto issue_s = [&](int j, int h) {
+          const int k_at = it1 + 2 * j;
+          if (!full(k_at, 125)) return;
+          tc_fence_after();
+          issue_nt(tmem + h * 64, res, ring + (k_at % kRing) * kStep + h * kHalfRows, ksteps, attn_idesc(kFmt, keys(j, h), false));
+          mma_commit(&s.s_full[h]);
+        };
+        auto issue_dp = [&](int j, int h) {
+          const int v_at = it1 + 2 * j + 1;
+          if (!full(v_at, 127)) return;
+          tc_fence_after();
+          issue_nt(tmem + 128 + h * 64, res + kStep, ring + (v_at % kRing) * kStep + h * kHalfRows, ksteps,
+                   attn_idesc(kFmt, keys(j, h), false));
+          mma_commit(&s.dp_full[h]);
+        };
+        auto issue_dq = [&](int j, int h) {
+          const int k_at = it1 + 2 * j;
+          tc_fence_after();
+          issue_tn<4>(tmem + 384, tmem + 256 + h * 32, 0, ring_mn + (k_at % kRing) * kStep + h * kHalfRows, keys(j, h) / 16, id_o,
+                      (j > 0 || h > 0) ? 1u : 0u);
+          mma_commit(&s.ds_free[h]);
+        };
+        // the ends of a key tile: its V has been read by both halves' dP, its K by both halves' dQ
+        auto end_v = [&](int j) {
+          mma_commit(&s.empty[(it1 + 2 * j + 1) % kRing]);
+          if (j + 1 == w.n_t) mma_commit(&s.res_empty);
+        };
+        auto end_k = [&](int j) {
+          mma_commit(&s.empty[(it1 + 2 * j) % kRing]);
+          if (j + 1 == w.n_t) mma_commit(&s.acc_done);
+        };
+        wait(&s.res_full, static_cast<uint32_t>(cnt), 123);
+        for (int h = 0; h < 2; ++h)
+          if (n_h[h] > 0 && ok) issue_s(0, h);
+        for (int h = 0; h < 2; ++h)
+          if (n_h[h] > 0 && ok) issue_dp(0, h);
+        if (w.o || kHalf) {  // the rows' dO and O have been read: before either tile may be overwritten
+          if (wait(&s.o_read, static_cast<uint32_t>(o_cnt), 133) && w.o) mbar_arrive(&s.empty[it % kRing]);
+        }
+        if (ok) end_v(0);
+        for (int j = 0; j < w.n_t && ok; ++j) {
+          const bool more0 = j + 1 < n_h[0], more1 = j + 1 < n_h[1];
+          // half 1 has dS(j - 1); first, because K(j + 1) may need the place of K(j - 1)
+          if (j > 0) {
+            if (!wait(&s.ds_full[1], done[1] + j - 1, 126)) break;
+            issue_dq(j - 1, 1);
+            end_k(j - 1);
+            if (j < n_h[1]) issue_dp(j, 1);
             if (!ok) break;
+            end_v(j);
           }
-          if (more) {
-            ok = mbar_wait(&s.full[k_next % kRing], (k_next / kRing) & 1, abort_flag, a.sink, 125);
-            if (!ok) break;
-            tc_fence_after();
-            issue_nt(tmem, res, ring + (k_next % kRing) * kStep, ksteps, id_s);
-            mma_commit(&s.s_full);
+          // half 0 has S(j) in registers
+          if (!wait(&s.p_full[0], done[0] + j, 124)) break;
+          if (more0) issue_s(j + 1, 0);
+          // half 0 has dS(j)
+          if (!wait(&s.ds_full[0], done[0] + j, 134)) break;
+          issue_dq(j, 0);
+          if (more0) issue_dp(j + 1, 0);
+          // half 1 has S(j) in registers
+          if (j < n_h[1]) {
+            if (!wait(&s.p_full[1], done[1] + j, 135)) break;
+            if (more1) issue_s(j + 1, 1);
           }
-          if (j >= 0) {  // dQ += dS(j) K(j)
-            ok = mbar_wait(&s.ds_full, (done + j) & 1, abort_flag, a.sink, 126);
-            if (!ok) break;
-            tc_fence_after();
-            issue_tn(tmem + 384, tmem + 256, 32, ring_mn + (k_at % kRing) * kStep, 8, id_o, j > 0 ? 1u : 0u);
-            mma_commit(&s.ds_free);
-            mma_commit(&s.empty[k_at % kRing]);
-            if (!more) mma_commit(&s.acc_done);
+        }
+        if (ok) {
+          if (n_h[1] == w.n_t) {
+            if (wait(&s.ds_full[1], done[1] + w.n_t - 1, 136)) issue_dq(w.n_t - 1, 1);
           }
-          if (more) {  // dP(j + 1): dP(j) was in registers before dS(j) was ready
-            ok = mbar_wait(&s.full[v_next % kRing], (v_next / kRing) & 1, abort_flag, a.sink, 127);
-            if (!ok) break;
-            tc_fence_after();
-            issue_nt(tmem + 128, res + kStep, ring + (v_next % kRing) * kStep, ksteps, id_s);
-            mma_commit(&s.dp_full);
-            mma_commit(&s.empty[v_next % kRing]);
-            if (j + 2 == w.n_t) mma_commit(&s.res_empty);
-          }
+          if (ok) end_k(w.n_t - 1);
         }
       }
       ok = __all_sync(0xffffffffu, ok);
-      it += 2 * w.n_t;
-      done += w.n_t;
+      it += w.o + 2 * w.n_t;
+      done[0] += w.n_t;
+      done[1] += w.n1;
+      o_cnt += (w.o || kHalf) ? 1 : 0;
       ++cnt;
     }
     __syncwarp();
@@ -193,41 +282,50 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t t_s = tmem + lanes + half * 64, t_dp = t_s + 128, t_ds = tmem + lanes + 256 + half * 32, t_dq = tmem + lanes + 384;
     uint8_t* stage = s.out[warp];
-    uint32_t cnt = 0;  // key tiles so far: the phase of every per-tile barrier
-    uint32_t done = 0;
+    uint32_t cnt = 0;  // key tiles of this half so far: the phase of every per-tile barrier
+    uint32_t items = 0, swaps = 0;
     int it = 0;
     bool ok = true;
     for (int item = blockIdx.x; item < a.items && ok; item += gridDim.x) {
       const Item w = get(item);
-      const int it0 = it;
-      it += 2 * w.n_t;
+      const int it1 = it + w.o;
       const int row = w.qt * kTile + r;
       const long long at = (static_cast<long long>(w.b) * a.s.hb + w.hb) * a.s.rows_pad + row;
-      float lse = INFINITY, delta = 0.f;
-      if (row < a.s.rows && w.n_t > 0) {
-        lse = a.lse[at];
-        const int pos = row / a.s.gp, head = w.hb * a.s.gp + row % a.s.gp;
-        const uint4* po = reinterpret_cast<const uint4*>(
-            static_cast<const T*>(a.out) + ((static_cast<long long>(w.b) * a.s.sq + pos) * a.s.hq + head) * a.s.d);
-        const uint4* pg = reinterpret_cast<const uint4*>(
-            static_cast<const T*>(a.dout) + w.b * a.do_b + pos * a.do_s + head * a.do_h);
-        for (int v = 0; v < a.s.d / 8; ++v) {
-          const uint4 x = __ldg(po + v), y = __ldg(pg + v);
-          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+      float nlse = -INFINITY, ndelta = 0.f, peak = 0.f;
+      if (w.n_t > 0) {
+        nlse = __ldg(a.lse + at);
+        if (w.o || kHalf) {  // the row's dO (and O), 16 bytes of each at a time; chunk c of row r lies at c ^ (r & 7)
+          ok = warp_wait(&s.res_full, items & 1, abort_flag, a.sink, 137);
+          if (ok && w.o) ok = warp_wait(&s.full[it % kRing], (it / kRing) & 1, abort_flag, a.sink, 138);
+          if (!ok) break;
+          for (int c = 0; c < a.s.d / 8; ++c) {
+            const int off = (c >> 3) * kBlkBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+            const uint4 g = *reinterpret_cast<const uint4*>(s.res[1] + off);
+            if constexpr (kHalf) peak = peak8<T>(g, peak);
+            if (w.o) {
+              const uint4 o = *reinterpret_cast<const uint4*>(s.ring[it % kRing] + off);
+              const uint32_t gs[4] = {g.x, g.y, g.z, g.w}, os[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 fx = unpack_pair<T>(xs[e]), fy = unpack_pair<T>(ys[e]);
-            delta = fmaf(fx.x, fy.x, delta);
-            delta = fmaf(fx.y, fy.y, delta);
+              for (int e = 0; e < 4; ++e) {
+                const float2 fg = unpack_pair<T>(gs[e]), fo = unpack_pair<T>(os[e]);
+                ndelta = fmaf(-fg.x, fo.x, ndelta);
+                ndelta = fmaf(-fg.y, fo.y, ndelta);
+              }
+            }
           }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s.o_read);
         }
+        ++items;
       }
-      if (half == 0) a.delta[at] = delta;
-      for (int j = 0; j < w.n_t; ++j, ++cnt) {
+      const float factor = kHalf ? grad_factor(peak) : 1.f;
+      const int mine = half == 0 ? w.n_t : w.n1;
+      const uint64_t c2 = f2_pack(a.c, a.c), nlse2 = f2_pack(nlse, nlse);
+      for (int j = 0; j < mine; ++j, ++cnt) {
         uint32_t bits[4];
-        const bool partial = key_bits(a.mask, w.b, a.s.sk, w.n_keys, j, lane, bits);
-        const uint32_t b0 = half == 0 ? bits[0] : bits[2], b1 = half == 0 ? bits[1] : bits[3];
-        ok = warp_wait(&s.s_full, cnt & 1, abort_flag, a.sink, 128);
+        const bool partial = (a.mask.key_mask != nullptr || (j + 1) * kTile > w.n_keys) &&
+                             key_bits(a.mask, w.b, a.s.sk, w.n_keys, j, lane, bits);
+        ok = warp_wait(&s.s_full[half], cnt & 1, abort_flag, a.sink, 128);
         if (!ok) break;
         tc_fence_after();
         float p[2][32];
@@ -236,47 +334,72 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         tc_wait_ld();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s.p_full);
+        if (lane == 0) mbar_arrive(&s.p_full[half]);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int e = 0; e < 32; ++e) p[i][e] = ex2_approx(fmaf(p[i][e], a.c, -lse));
-        if (partial) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            p[0][e] = (b0 >> e) & 1u ? p[0][e] : 0.f;
-            p[1][e] = (b1 >> e) & 1u ? p[1][e] : 0.f;
+          for (int e = 0; e < 32; e += 2) {
+            const float2 y = f2_unpack(f2_fma(f2_pack(p[i][e], p[i][e + 1]), c2, nlse2));
+            p[i][e] = ex2_approx(y.x);
+            p[i][e + 1] = ex2_approx(y.y);
           }
-          if (half == 0) {  // see the forward pass: a masked key's row of K must not reach the last product
-            const int k_at = it0 + 2 * j;
-            ok = warp_wait(&s.full[k_at % kRing], (k_at / kRing) & 1, abort_flag, a.sink, 129);
-            if (!ok) break;
-            if (!((bits[quarter] >> lane) & 1u)) clear_row<NB>(s.ring[k_at % kRing], r);
-            fence_proxy_async_smem();
-          }
-        }
-        ok = warp_wait(&s.dp_full, cnt & 1, abort_flag, a.sink, 130);
+        ok = warp_wait(&s.dp_full[half], cnt & 1, abort_flag, a.sink, 130);
         if (!ok) break;
         tc_fence_after();
         float dp[2][32];
         tc_ld32(t_dp, dp[0]);
         tc_ld32(t_dp + 32, dp[1]);
         tc_wait_ld();
-        if (partial) {  // dP of a masked key may be anything, NaN included
+        if (partial) {  // S and dP of a masked key may be anything, NaN included
+          const uint32_t b0 = half == 0 ? bits[0] : bits[2], b1 = half == 0 ? bits[1] : bits[3];
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
+            p[0][e] = (b0 >> e) & 1u ? p[0][e] : 0.f;
+            p[1][e] = (b1 >> e) & 1u ? p[1][e] : 0.f;
             dp[0][e] = (b0 >> e) & 1u ? dp[0][e] : 0.f;
             dp[1][e] = (b1 >> e) & 1u ? dp[1][e] : 0.f;
           }
+          // ... and its row of K must not reach the last product: this half's 64 rows, two threads each
+          const int k_at = it1 + 2 * j;
+          ok = warp_wait(&s.full[k_at % kRing], (k_at / kRing) & 1, abort_flag, a.sink, 129);
+          if (!ok) break;
+          const int key = half * 64 + (r & 63);
+          const uint32_t word = (r & 32) ? b1 : b0;
+          if (r < 64 && !((word >> lane) & 1u)) clear_row<NB>(s.ring[k_at % kRing], key);
+          fence_proxy_async_smem();
+        }
+        if (!w.o) {  // one key tile: delta = sum of P dP over the row's keys, both halves'
+          uint64_t acc = 0;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) acc = f2_fma(f2_pack(p[i][e], p[i][e + 1]), f2_pack(dp[i][e], dp[i][e + 1]), acc);
+          const float2 v = f2_unpack(acc);
+          float sum = v.x + v.y;
+          if (w.n1 > 0) {
+            s.red[swaps & 1][half][r] = sum;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.pair[quarter]);
+            ok = warp_wait(&s.pair[quarter], swaps & 1, abort_flag, a.sink, 139);
+            if (!ok) break;
+            sum = s.red[swaps & 1][0][r] + s.red[swaps & 1][1][r];
+            ++swaps;
+          }
+          ndelta = -sum;
         }
         uint32_t pk[32];
+        const uint64_t nd2 = f2_pack(ndelta * factor, ndelta * factor), factor2 = f2_pack(factor, factor);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int e = 0; e < 32; e += 2)
-            pk[i * 16 + e / 2] = pack2<T>(p[i][e] * (dp[i][e] - delta), p[i][e + 1] * (dp[i][e + 1] - delta));
+          for (int e = 0; e < 32; e += 2) {
+            const uint64_t x = f2_pack(dp[i][e], dp[i][e + 1]);
+            const uint64_t d = kHalf ? f2_fma(x, factor2, nd2) : f2_add(x, nd2);
+            const float2 ds = f2_unpack(f2_mul(f2_pack(p[i][e], p[i][e + 1]), d));
+            pk[i * 16 + e / 2] = pack2<T>(ds.x, ds.y);
+          }
         if (cnt > 0) {
-          ok = warp_wait(&s.ds_free, (cnt - 1) & 1, abort_flag, a.sink, 131);
+          ok = warp_wait(&s.ds_free[half], (cnt - 1) & 1, abort_flag, a.sink, 131);
           if (!ok) break;
           tc_fence_after();
         }
@@ -284,22 +407,27 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s.ds_full);
+        if (lane == 0) mbar_arrive(&s.ds_full[half]);
       }
       if (!ok) break;
+      it = it1 + 2 * w.n_t;
+      if (half == 0) {
+        a.delta[at] = ndelta;
+        if constexpr (kHalf) a.peak[at] = peak;
+      }
       if (w.n_t > 0) {
-        ok = warp_wait(&s.acc_done, done & 1, abort_flag, a.sink, 132);
+        ok = warp_wait(&s.acc_done, (items - 1) & 1, abort_flag, a.sink, 132);
         if (!ok) break;
-        ++done;
         tc_fence_after();
       }
       const int pos = w.qt * pos_per_tile + quarter * 32 / a.s.gp;
+      const float mul = a.scale / factor;
       for (int c = half * 32; c < a.s.d; c += 64) {
         float o[32];
         tc_ld32(t_dq + c, o);
         tc_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = w.n_t == 0 ? 0.f : o[e] * a.scale;
+        for (int e = 0; e < 32; ++e) o[e] = w.n_t == 0 ? 0.f : o[e] * mul;
         store_block<T>(&map_dq, stage, o, lane, c, w.hb * a.s.gp, pos, w.b, pos < a.s.sq);
       }
       tc_fence_before();
@@ -322,6 +450,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 const __grid_constant__ CUtensorMap map_dk, const __grid_constant__ CUtensorMap map_dv, const BwdArgs a) {
   constexpr int kRing = BwdSmem<NB>::kRing;
   constexpr int kTileBytes = NB * kBlkBytes;
+  constexpr bool kHalf = std::is_same<T, __half>::value;
   extern __shared__ uint8_t smem_raw[];
   BwdSmem<NB>& s = *reinterpret_cast<BwdSmem<NB>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -393,9 +522,10 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     if (!ok) settle();
   } else if (warp == 9) {
     const int ksteps = a.s.dn / 16;
-    const uint32_t id_s = attn_idesc(kFmt, kTile, false), id_o = attn_idesc(kFmt, a.s.dn, true);
+    const uint32_t id_s = attn_idesc(kFmt, 64, false), id_o = attn_idesc(kFmt, a.s.dn, true);
     const uint64_t res = desc_k(smem_u32(s.res[0])), ring = desc_k(smem_u32(s.ring[0])), ring_mn = desc_mn<>(smem_u32(s.ring[0]));
     constexpr uint32_t kStep = kTileBytes >> 4;
+    constexpr uint32_t kHalfRows = 64 * 128 >> 4;  // the second half of a tile's rows
     int it = 0, cnt = 0;
     uint32_t done = 0;  // query tiles of the items before
     bool ok = true;
@@ -403,40 +533,60 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       const Item w = get(item);
       if (w.n_i == 0) continue;
       if (elect_one()) {
-        ok = mbar_wait(&s.res_full, cnt & 1, abort_flag, a.sink, 144);
-        for (int i = -1; i < w.n_i && ok; ++i) {
-          const int qa = it + 2 * i, da = qa + 1, qn = qa + 2, dn = qa + 3;
+        auto wait = [&](uint64_t* bar, uint32_t n, int code) {
+          if (ok) ok = mbar_wait(bar, n & 1, abort_flag, a.sink, code);
+          return ok;
+        };
+        auto full = [&](int at, int code) { return wait(&s.full[at % kRing], static_cast<uint32_t>(at / kRing), code); };
+        auto issue_s = [&](int i, int h) {
+          const int q_at = it + 2 * i;
+          if (!full(q_at, 146)) return;
+          tc_fence_after();
+          issue_nt(tmem + h * 64, res, ring + (q_at % kRing) * kStep + h * kHalfRows, ksteps, id_s);
+          mma_commit(&s.s_full[h]);
+        };
+        auto issue_dp = [&](int i, int h) {
+          const int d_at = it + 2 * i + 1;
+          if (!full(d_at, 148)) return;
+          tc_fence_after();
+          issue_nt(tmem + 128 + h * 64, res + kStep, ring + (d_at % kRing) * kStep + h * kHalfRows, ksteps, id_s);
+          mma_commit(&s.dp_full[h]);
+          if (h == 1 && i + 1 == w.n_i) mma_commit(&s.res_empty);
+        };
+        // acc += A(i) of half h times the rows of that half of the tile in ring position `at`
+        auto issue_acc = [&](uint32_t acc, uint32_t src, int at, int i, int h) {
+          tc_fence_after();
+          issue_tn<4>(acc, src + h * 64, 0, ring_mn + (at % kRing) * kStep + h * kHalfRows, 4, id_o, (i > 0 || h > 0) ? 1u : 0u);
+        };
+        wait(&s.res_full, static_cast<uint32_t>(cnt), 144);
+        for (int h = 0; h < 2; ++h)
+          if (ok) issue_s(0, h);
+        for (int h = 0; h < 2; ++h)
+          if (ok) issue_dp(0, h);
+        for (int i = 0; i < w.n_i && ok; ++i) {
+          const int q_at = it + 2 * i, d_at = q_at + 1;
           const bool more = i + 1 < w.n_i;
-          if (i >= 0) {  // dV += P(i) dO(i)
-            ok = mbar_wait(&s.p_full, (done + i) & 1, abort_flag, a.sink, 145);
-            if (!ok) break;
-            tc_fence_after();
-            issue_tn(tmem + 256, tmem, 64, ring_mn + (da % kRing) * kStep, 8, id_o, i > 0 ? 1u : 0u);
-            mma_commit(&s.empty[da % kRing]);
+          if (i > 0) {  // first, because Q(i + 1) may need the place of Q(i - 1)
+            if (!wait(&s.ds_full[1], done + i - 1, 147)) break;
+            issue_acc(tmem + 384, tmem + 128, q_at - 2, i - 1, 1);
+            mma_commit(&s.empty[(q_at - 2) % kRing]);  // Q(i - 1)
+            issue_dp(i, 1);
           }
-          if (more) {  // S(i + 1) over P(i), which dV(i) reads first
-            ok = mbar_wait(&s.full[qn % kRing], (qn / kRing) & 1, abort_flag, a.sink, 146);
-            if (!ok) break;
-            tc_fence_after();
-            issue_nt(tmem, res, ring + (qn % kRing) * kStep, ksteps, id_s);
-            mma_commit(&s.s_full);
-          }
-          if (i >= 0) {  // dK += dS(i) Q(i)
-            ok = mbar_wait(&s.ds_full, (done + i) & 1, abort_flag, a.sink, 147);
-            if (!ok) break;
-            tc_fence_after();
-            issue_tn(tmem + 384, tmem + 128, 64, ring_mn + (qa % kRing) * kStep, 8, id_o, i > 0 ? 1u : 0u);
-            mma_commit(&s.empty[qa % kRing]);
-            if (!more) mma_commit(&s.acc_done);
-          }
-          if (more) {
-            ok = mbar_wait(&s.full[dn % kRing], (dn / kRing) & 1, abort_flag, a.sink, 148);
-            if (!ok) break;
-            tc_fence_after();
-            issue_nt(tmem + 128, res + kStep, ring + (dn % kRing) * kStep, ksteps, id_s);
-            mma_commit(&s.dp_full);
-            if (i + 2 == w.n_i) mma_commit(&s.res_empty);
-          }
+          if (!wait(&s.p_full[0], done + i, 145)) break;
+          issue_acc(tmem + 256, tmem, d_at, i, 0);  // dV += P(i) dO(i), then S(i + 1) over P(i)
+          if (more) issue_s(i + 1, 0);
+          if (!wait(&s.ds_full[0], done + i, 153)) break;
+          issue_acc(tmem + 384, tmem + 128, q_at, i, 0);  // dK += dS(i) Q(i), then dP(i + 1) over dS(i)
+          if (more) issue_dp(i + 1, 0);
+          if (!wait(&s.p_full[1], done + i, 154)) break;
+          issue_acc(tmem + 256, tmem, d_at, i, 1);
+          mma_commit(&s.empty[d_at % kRing]);  // dO(i)
+          if (more) issue_s(i + 1, 1);
+        }
+        if (wait(&s.ds_full[1], done + w.n_i - 1, 155)) {
+          issue_acc(tmem + 384, tmem + 128, it + 2 * (w.n_i - 1), w.n_i - 1, 1);
+          mma_commit(&s.empty[(it + 2 * (w.n_i - 1)) % kRing]);
+          mma_commit(&s.acc_done);
         }
       }
       ok = __all_sync(0xffffffffu, ok);
@@ -463,59 +613,90 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         key_bits(a.mask, w.b, a.s.sk, w.n_keys, w.kt, lane, bits);
         mine = (bits[quarter] >> lane) & 1u;
       }
+      float factor = 1.f;  // fp16: on dS
+      if constexpr (kHalf) {
+        if (w.n_i > 0) {
+          float top = 0.f;
+          for (int i = 0; i < w.n_i; ++i) {
+            const int sub = (w.i0 + i) / a.s.qtiles, qt = (w.i0 + i) - sub * a.s.qtiles;
+            const float4 v = __ldg(reinterpret_cast<const float4*>(
+                a.peak + (static_cast<long long>(w.b) * a.s.hb + w.h * group_blocks + sub) * a.s.rows_pad + qt * kTile) + lane);
+            top = max3(max3(top, v.x, v.y), v.z, v.w);
+          }
+#pragma unroll
+          for (int d = 16; d >= 1; d >>= 1) top = max3(top, __shfl_xor_sync(0xffffffffu, top, d), top);
+          factor = grad_factor(top);
+        }
+      }
+      const float p_up = kHalf ? exp2f(a.p_shift) : 1.f;
+      const uint64_t c2 = f2_pack(a.c, a.c), shift2 = f2_pack(a.p_shift, a.p_shift);
+      const uint64_t f2 = f2_pack(factor / p_up, factor / p_up);
+      const bool any = __any_sync(0xffffffffu, mine);  // rows of a warp without keys stay as they are: zeros are written
       for (int i = 0; i < w.n_i; ++i, ++cnt) {
         const int qa = it0 + 2 * i;
         ok = warp_wait(&s.full[qa % kRing], (qa / kRing) & 1, abort_flag, a.sink, 149);  // the statistics have landed
         if (!ok) break;
-        const float4* st_l = reinterpret_cast<const float4*>(s.stat[(qa % kRing) / 2][0]) + half * 16;
-        const float4* st_d = reinterpret_cast<const float4*>(s.stat[(qa % kRing) / 2][1]) + half * 16;
-        ok = warp_wait(&s.s_full, cnt & 1, abort_flag, a.sink, 150);
+        const ulonglong2* st_l = reinterpret_cast<const ulonglong2*>(s.stat[(qa % kRing) / 2][0]) + half * 16;
+        const ulonglong2* st_d = reinterpret_cast<const ulonglong2*>(s.stat[(qa % kRing) / 2][1]) + half * 16;
+        ok = warp_wait(&s.s_full[half], cnt & 1, abort_flag, a.sink, 150);
         if (!ok) break;
         tc_fence_after();
         float p[2][32];
-        tc_ld32(t_s, p[0]);
-        tc_ld32(t_s + 32, p[1]);
-        tc_wait_ld();
         uint32_t pk[32];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            const float4 l4 = st_l[h * 8 + e / 4];
-            p[h][e] = ex2_approx(fmaf(p[h][e], a.c, -l4.x));
-            p[h][e + 1] = ex2_approx(fmaf(p[h][e + 1], a.c, -l4.y));
-            p[h][e + 2] = ex2_approx(fmaf(p[h][e + 2], a.c, -l4.z));
-            p[h][e + 3] = ex2_approx(fmaf(p[h][e + 3], a.c, -l4.w));
-            pk[h * 16 + e / 2] = mine ? pack2<T>(p[h][e], p[h][e + 1]) : 0u;
-            pk[h * 16 + e / 2 + 1] = mine ? pack2<T>(p[h][e + 2], p[h][e + 3]) : 0u;
-          }
-        tc_st32(t_s, pk);
-        tc_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s.p_full);
-        ok = warp_wait(&s.dp_full, cnt & 1, abort_flag, a.sink, 151);
-        if (!ok) break;
-        tc_fence_after();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float dp[32];
-          tc_ld32(t_dp + h * 32, dp);
+        if (any) {
+          tc_ld32(t_s, p[0]);
+          tc_ld32(t_s + 32, p[1]);
           tc_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            const float4 d4 = st_d[h * 8 + e / 4];
-            const uint32_t lo = pack2<T>(p[h][e] * (dp[e] - d4.x), p[h][e + 1] * (dp[e + 1] - d4.y));
-            const uint32_t hi = pack2<T>(p[h][e + 2] * (dp[e + 2] - d4.z), p[h][e + 3] * (dp[e + 3] - d4.w));
-            pk[h * 16 + e / 2] = mine ? lo : 0u;
-            pk[h * 16 + e / 2 + 1] = mine ? hi : 0u;
-          }
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const ulonglong2 l4 = st_l[h * 8 + e / 4];
+              const uint64_t la = kHalf ? f2_add(l4.x, shift2) : l4.x, lb = kHalf ? f2_add(l4.y, shift2) : l4.y;
+              const float2 ya = f2_unpack(f2_fma(f2_pack(p[h][e], p[h][e + 1]), c2, la));
+              const float2 yb = f2_unpack(f2_fma(f2_pack(p[h][e + 2], p[h][e + 3]), c2, lb));
+              p[h][e] = ex2_approx(ya.x);
+              p[h][e + 1] = ex2_approx(ya.y);
+              p[h][e + 2] = ex2_approx(yb.x);
+              p[h][e + 3] = ex2_approx(yb.y);
+              pk[h * 16 + e / 2] = pack2<T>(p[h][e], p[h][e + 1]);
+              pk[h * 16 + e / 2 + 1] = pack2<T>(p[h][e + 2], p[h][e + 3]);
+            }
+          tc_st32(t_s, pk);
+          tc_wait_st();
         }
-        tc_st32(t_dp, pk);
-        tc_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s.ds_full);
+        if (lane == 0) mbar_arrive(&s.p_full[half]);
+        ok = warp_wait(&s.dp_full[half], cnt & 1, abort_flag, a.sink, 151);
+        if (!ok) break;
+        tc_fence_after();
+        if (any) {
+          float dp[2][32];
+          tc_ld32(t_dp, dp[0]);
+          tc_ld32(t_dp + 32, dp[1]);
+          tc_wait_ld();
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const ulonglong2 d4 = st_d[h * 8 + e / 4];
+              uint64_t da = f2_add(f2_pack(dp[h][e], dp[h][e + 1]), d4.x), db = f2_add(f2_pack(dp[h][e + 2], dp[h][e + 3]), d4.y);
+              if constexpr (kHalf) {
+                da = f2_mul(da, f2);
+                db = f2_mul(db, f2);
+              }
+              const float2 sa = f2_unpack(f2_mul(f2_pack(p[h][e], p[h][e + 1]), da));
+              const float2 sb = f2_unpack(f2_mul(f2_pack(p[h][e + 2], p[h][e + 3]), db));
+              pk[h * 16 + e / 2] = pack2<T>(sa.x, sa.y);
+              pk[h * 16 + e / 2 + 1] = pack2<T>(sb.x, sb.y);
+            }
+          tc_st32(t_dp, pk);
+          tc_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.ds_full[half]);
       }
       if (!ok) break;
       if (w.n_i > 0) {
@@ -528,13 +709,13 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       const int key = w.kt * kTile + r;
       for (int which = 0; which < 2; ++which) {
         const uint32_t src = which == 0 ? t_dv : t_dk;
-        const float mul = which == 0 ? 1.f : a.scale;
+        const float mul = which == 0 ? 1.f / p_up : a.scale / factor;
         for (int c = half * 32; c < a.s.d; c += 64) {
           float o[32];
           tc_ld32(src + c, o);
           tc_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = w.n_i == 0 ? 0.f : o[e] * mul;
+          for (int e = 0; e < 32; ++e) o[e] = mine ? o[e] * mul : 0.f;
           if (a.splits > 1) {
             const long long n = static_cast<long long>(a.s.batch) * a.s.sk * a.s.hkv;
             const long long at = (static_cast<long long>(w.b) * a.s.sk + key) * a.s.hkv + w.h;
@@ -595,11 +776,11 @@ static void bwd_plan(BwdArgs& a) {
   a.splits = (a.steps + a.steps_per_split - 1) / a.steps_per_split;
 }
 
-static size_t bwd_delta_bytes(const AttnShape& s) {
-  return static_cast<size_t>(s.batch) * s.hb * s.rows_pad * sizeof(float);
+static size_t bwd_stat_bytes(const AttnShape& s) {  // delta, and the row peaks of fp16
+  return 2 * static_cast<size_t>(s.batch) * s.hb * s.rows_pad * sizeof(float);
 }
 static size_t bwd_ws(const BwdArgs& a) {
-  size_t n = bwd_delta_bytes(a.s);
+  size_t n = bwd_stat_bytes(a.s);
   if (a.splits > 1) n += static_cast<size_t>(a.splits) * 2 * a.s.batch * a.s.sk * a.s.hkv * a.s.d * sizeof(float);
   return n;
 }
@@ -658,16 +839,16 @@ int nd_attn_bwd(int dtype, const void* dout, const void* q, const void* k, const
   a.sink = WaitSink{nullptr, device_error_ptr()};
   a.lse = lse;
   a.delta = static_cast<float*>(ws);
-  a.part = reinterpret_cast<float*>(static_cast<char*>(ws) + bwd_delta_bytes(a.s));
-  a.out = out;
-  a.dout = dout;
-  a.do_b = strides[9]; a.do_s = strides[10]; a.do_h = strides[11];
+  a.peak = a.delta + static_cast<size_t>(a.s.batch) * a.s.hb * a.s.rows_pad;
+  a.part = reinterpret_cast<float*>(static_cast<char*>(ws) + bwd_stat_bytes(a.s));
+  for (int n = a.s.sk; dtype == ND_F16 && n > 1 && a.p_shift < 12.f; n >>= 1) a.p_shift += 1.f;
   a.scale = scale;
   a.c = scale * 1.4426950408889634f;
-  CUtensorMap mq, mdo, mk, mv, mdq, mdk, mdv;
+  CUtensorMap mq, mdo, mo, mk, mv, mdq, mdk, mdv;
   const int64_t ro = hq * head_dim, rk = hkv * head_dim;
   if (!attn_map(&mq, dtype, q, batch, sq, hq, head_dim, strides[0], strides[1], strides[2], 64, a.s.gp, kTile / a.s.gp) ||
       !attn_map(&mdo, dtype, dout, batch, sq, hq, head_dim, strides[9], strides[10], strides[11], 64, a.s.gp, kTile / a.s.gp) ||
+      !attn_map(&mo, dtype, out, batch, sq, hq, head_dim, sq * ro, ro, head_dim, 64, a.s.gp, kTile / a.s.gp) ||
       !attn_map(&mk, dtype, k, batch, sk, hkv, head_dim, strides[3], strides[4], strides[5], 64, 1, kTile) ||
       !attn_map(&mv, dtype, v, batch, sk, hkv, head_dim, strides[6], strides[7], strides[8], 64, 1, kTile) ||
       !attn_map(&mdq, dtype, dq, batch, sq, hq, head_dim, sq * ro, ro, head_dim, 32, a.s.gp, 32 / a.s.gp) ||
@@ -682,7 +863,7 @@ int nd_attn_bwd(int dtype, const void* dout, const void* q, const void* k, const
   const void* f2 = one ? (bf ? (const void*)attn_dkv_kernel<1, __nv_bfloat16> : (const void*)attn_dkv_kernel<1, __half>)
                        : (bf ? (const void*)attn_dkv_kernel<2, __nv_bfloat16> : (const void*)attn_dkv_kernel<2, __half>);
   a.items = static_cast<int>(q_items);
-  void* p1[] = {&mq, &mdo, &mk, &mv, &mdq, &a};
+  void* p1[] = {&mq, &mdo, &mo, &mk, &mv, &mdq, &a};
   int e = attn_launch(f1, a.items < sms ? a.items : sms, kBwdThreads, smem, p1, st);
   if (e != ND_OK) return e;
   a.items = static_cast<int>(k_items);

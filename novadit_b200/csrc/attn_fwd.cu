@@ -50,7 +50,7 @@ struct FwdArgs {
   AttnShape s;
   AttnMask mask;
   WaitSink sink;
-  float* lse;      // [batch, hb, rows_pad], log2 of the sum of 2^(score c); nullable
+  float* lse;      // [batch, hb, rows_pad], minus log2 of the sum of 2^(score c); nullable
   float* part_o;   // splits > 1: [splits][batch * hb][rows_pad][d], normalised
   float* part_l;   // splits > 1: [splits][batch * hb][rows_pad], -inf: no keys
   float c;         // scale * log2(e)
@@ -377,8 +377,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           }
         }
       } else {
-        if (a.lse != nullptr)  // +inf where there is nothing: 2^(s - inf) = 0 in the backward pass
-          a.lse[head_row * a.s.rows_pad + row] = (l == 0.f || row >= a.s.rows) ? INFINITY : m * a.c + log2f(l);
+        if (a.lse != nullptr)  // -inf where there is nothing: 2^(s - inf) = 0 in the backward pass
+          a.lse[head_row * a.s.rows_pad + row] = (l == 0.f || row >= a.s.rows) ? -INFINITY : -(m * a.c + log2f(l));
         const int pos = (2 * w.pair + t) * pos_per_tile + quarter * 32 / a.s.gp;
         for (int c = 0; c < a.s.d; c += 32) {
           float o[2][16];
@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const FwdArgs a, T* __re
       acc.w = fmaf(wgt, o.w, acc.w);
     }
   }
-  if (lane == 0 && a.lse != nullptr) a.lse[at] = (total == 0.f || row >= a.s.rows) ? INFINITY : top + log2f(total);
+  if (lane == 0 && a.lse != nullptr) a.lse[at] = (total == 0.f || row >= a.s.rows) ? -INFINITY : -(top + log2f(total));
   if (row >= a.s.rows || lane * 4 >= a.s.d) return;
   const float inv = total == 0.f ? 0.f : 1.f / total;
   const int b = static_cast<int>(head_row / a.s.hb), hb = static_cast<int>(head_row - static_cast<long long>(b) * a.s.hb);
