@@ -144,14 +144,15 @@ __device__ __forceinline__ void issue_nt(uint32_t d, uint64_t a, uint64_t b, int
   for (int k = 1; k < 8; ++k)
     if (k < steps) mma_ss(d, a + step_k(k), b + step_k<ROWS>(k), idesc, 1u);
 }
-// D (+)= A B over `steps` groups of 16 rows of B: A from tensor memory, `gap` columns between its steps 3 and 4
-template <int MAX = 8>
-__device__ __forceinline__ void issue_tn(uint32_t d, uint32_t a, uint32_t gap, uint64_t b, int steps, uint32_t idesc,
+// D (+)= A B over `steps` groups of 16 rows of B: A from tensor memory, 8 columns per step, every GROUP steps `stride` columns
+// behind the ones before
+template <int MAX, int GROUP>
+__device__ __forceinline__ void issue_tn(uint32_t d, uint32_t a, uint32_t stride, uint64_t b, int steps, uint32_t idesc,
                                          uint32_t accumulate) {
   mma_ts(d, a, b, idesc, accumulate);
 #pragma unroll
   for (int k = 1; k < MAX; ++k)
-    if (k < steps) mma_ts(d, a + (k >> 2) * gap + (k & 3) * 8, b + step_mn(k), idesc, 1u);
+    if (k < steps) mma_ts(d, a + (k / GROUP) * stride + (k % GROUP) * 8, b + step_mn(k), idesc, 1u);
 }
 
 // Keys of sample b that take part lie below the returned index (exactly those, without a key mask). Called by whole

@@ -6,13 +6,12 @@
 // kernel that adds dQ up in global memory, but every sum stays in tensor memory in one fixed order: no atomics, results
 // do not change from run to run, and the second operand of every product is a tile that lies in shared memory already.
 //
-// Both: one persistent CTA per SM, 320 threads, warps 0-3 and 4-7 the elementwise part (a thread per row, each warpgroup
-// with 64 of the tile's 128 columns), warp 8 copies, warp 9 issues the MMAs. Each half of the columns has products and
-// barriers of its own, and the issuing thread takes them half a step apart: while one warpgroup waits for its products
-// the other computes (as one group of eight warps in step, a tile of 128 x 128 took 2800 cycles for dQ and 3300 for dK and
-// dV at D = 64, where the exponentials take 1024). P and dS are the A operands of the last products straight from
-// tensor memory, in 16 bits (one rounding, unbiased, below that of the output); scores, dP, statistics and
-// accumulators stay in 32 bits.
+// Both: one persistent CTA per SM, 640 threads, warps 0-15 the elementwise part, warp 16 copies, warp 17 issues the MMAs (two
+// more complete its warpgroup, which hands registers over: 16 x 32 x 104 + 4 x 32 x 64 = 640 x 96). A thread has a row and
+// 32 of the tile's 128 columns. Each half of the columns (two warpgroups) has products and barriers of its own, and the
+// issuing thread takes the halves half a step apart: while one waits for its products the other computes. P and dS are
+// the A operands of the last products straight from tensor memory, in 16 bits (one rounding, unbiased, below that of the
+// output); scores, dP, statistics and accumulators stay in 32 bits.
 //
 // dQ kernel, per key tile j and half:  S(j) = Q K^T, dP(j) = dO V^T, dQ += dS(j) K. S(j + 1) is issued as soon as S(j) is
 // in registers, dP(j + 1) behind dQ(j). delta comes from the row's dO and O tiles - or, where a sample has one key tile,
@@ -29,7 +28,7 @@
 
 namespace nd {
 
-constexpr int kBwdThreads = 320;
+constexpr int kBwdThreads = 640;
 
 struct BwdArgs {
   AttnShape s;
@@ -49,7 +48,7 @@ template <int NB> struct __align__(1024) BwdSmem {
   static constexpr int kRing = NB == 1 ? 8 : 4;
   uint8_t res[2][NB * kBlkBytes];        // dQ: Q, dO; dK/dV: K, V
   uint8_t ring[kRing][NB * kBlkBytes];   // dQ: K, V, K, V, ...; dK/dV: Q, dO, ...
-  uint8_t out[8][2048];
+  uint8_t out[8][2048];                  // staging of the first half's warps, which write the results
   alignas(16) float stat[kRing / 2][2][kTile];  // dK/dV: log-sum-exp and delta of the query tile
   uint64_t res_full, res_empty;
   uint64_t full[kRing], empty[kRing];
@@ -58,8 +57,8 @@ template <int NB> struct __align__(1024) BwdSmem {
   uint64_t ds_free[2];              // dQ: dS has been read
   uint64_t acc_done;                // the accumulators are complete
   uint64_t o_read;                  // dQ: the elementwise warps have read dO and O
-  uint64_t pair[4];                 // dQ: both halves of 32 rows have written to `red`
-  float red[2][2][kTile];           // dQ: [exchange parity][half][row]
+  uint64_t swap[4];                 // dQ: the four warps of 32 rows have written to `red`
+  float red[2][4][kTile];           // dQ: [exchange parity][warpgroup][row]
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -74,13 +73,13 @@ template <int NB> __device__ __forceinline__ void bwd_init(BwdSmem<NB>& s) {
   for (int h = 0; h < 2; ++h) {
     mbar_init(&s.s_full[h], 1);
     mbar_init(&s.dp_full[h], 1);
-    mbar_init(&s.p_full[h], 4);
-    mbar_init(&s.ds_full[h], 4);
+    mbar_init(&s.p_full[h], 8);
+    mbar_init(&s.ds_full[h], 8);
     mbar_init(&s.ds_free[h], 1);
   }
-  for (int i = 0; i < 4; ++i) mbar_init(&s.pair[i], 2);
+  for (int i = 0; i < 4; ++i) mbar_init(&s.swap[i], 4);
   mbar_init(&s.acc_done, 1);
-  mbar_init(&s.o_read, 8);
+  mbar_init(&s.o_read, 16);
   s.abort_flag = 0;
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }
@@ -118,7 +117,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &s.abort_flag;
   if (threadIdx.x == 0) bwd_init<NB>(s);
-  if (warp == 9) tmem_alloc<512>(&s.tmem_base);
+  if (warp == 17) tmem_alloc<512>(&s.tmem_base);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -147,7 +146,9 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     return w;
   };
 
-  if (warp == 8) {
+  if (warp >= 16) {
+   reg_give<64>();
+   if (warp == 16) {
     int it = 0, cnt = 0;
     bool ok = true;
     for (int item = blockIdx.x; item < a.items && ok; item += gridDim.x) {
@@ -174,7 +175,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       ++cnt;
     }
     if (!ok) settle();
-  } else if (warp == 9) {
+   } else if (warp == 17) {
     const int ksteps = a.s.dn / 16;
     const uint32_t id_o = attn_idesc(kFmt, a.s.dn, true);
     const uint64_t res = desc_k(smem_u32(s.res[0])), ring = desc_k(smem_u32(s.ring[0])), ring_mn = desc_mn<>(smem_u32(s.ring[0]));
@@ -216,7 +217,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         auto issue_dq = [&](int j, int h) {
           const int k_at = it1 + 2 * j;
           tc_fence_after();
-          issue_tn<4>(tmem + 384, tmem + 256 + h * 32, 0, ring_mn + (k_at % kRing) * kStep + h * kHalfRows, keys(j, h) / 16, id_o,
+          issue_tn<4, 4>(tmem + 384, tmem + 256 + h * 32, 0, ring_mn + (k_at % kRing) * kStep + h * kHalfRows, keys(j, h) / 16, id_o,
                       (j > 0 || h > 0) ? 1u : 0u);
           mma_commit(&s.ds_free[h]);
         };
@@ -277,15 +278,26 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       ++cnt;
     }
     __syncwarp();
+   }
   } else {
-    const int half = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    reg_take<104>();
+    const int half = warp >> 3, sub = (warp >> 2) & 1, group = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t t_s = tmem + lanes + half * 64, t_dp = t_s + 128, t_ds = tmem + lanes + 256 + half * 32, t_dq = tmem + lanes + 384;
-    uint8_t* stage = s.out[warp];
+    const uint32_t t_s = tmem + lanes + group * 32, t_dp = t_s + 128, t_ds = tmem + lanes + 256 + group * 16, t_dq = tmem + lanes + 384;
     uint32_t cnt = 0;  // key tiles of this half so far: the phase of every per-tile barrier
-    uint32_t items = 0, swaps = 0;
+    uint32_t items = 0;
     int it = 0;
     bool ok = true;
+    // sum over the four threads of a row, once per item
+    auto exchange = [&](float v, float& sum) -> bool {
+      s.red[items & 1][group][r] = v;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.swap[quarter]);
+      if (!warp_wait(&s.swap[quarter], items & 1, abort_flag, a.sink, 139)) return false;
+      const float* red = s.red[items & 1][0] + r;
+      sum = (red[0] + red[kTile]) + (red[2 * kTile] + red[3 * kTile]);
+      return true;
+    };
     for (int item = blockIdx.x; item < a.items && ok; item += gridDim.x) {
       const Item w = get(item);
       const int it1 = it + w.o;
@@ -298,11 +310,11 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           ok = warp_wait(&s.res_full, items & 1, abort_flag, a.sink, 137);
           if (ok && w.o) ok = warp_wait(&s.full[it % kRing], (it / kRing) & 1, abort_flag, a.sink, 138);
           if (!ok) break;
-          for (int c = 0; c < a.s.d / 8; ++c) {
+          for (int c = kHalf ? 0 : group; c < a.s.d / 8; c += kHalf ? 1 : 4) {  // a quarter each; fp16 looks at the whole row
             const int off = (c >> 3) * kBlkBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
             const uint4 g = *reinterpret_cast<const uint4*>(s.res[1] + off);
             if constexpr (kHalf) peak = peak8<T>(g, peak);
-            if (w.o) {
+            if (w.o && (!kHalf || (c & 3) == group)) {
               const uint4 o = *reinterpret_cast<const uint4*>(s.ring[it % kRing] + off);
               const uint32_t gs[4] = {g.x, g.y, g.z, g.w}, os[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
@@ -316,94 +328,79 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           __syncwarp();
           if (lane == 0) mbar_arrive(&s.o_read);
         }
-        ++items;
+        if (w.o || (half == 1 && w.n1 == 0)) {  // (the second: nothing to add to the one tile's sum below)
+          ok = exchange(ndelta, ndelta);
+          if (!ok) break;
+        }
       }
       const float factor = kHalf ? grad_factor(peak) : 1.f;
       const int mine = half == 0 ? w.n_t : w.n1;
       const uint64_t c2 = f2_pack(a.c, a.c), nlse2 = f2_pack(nlse, nlse);
       for (int j = 0; j < mine; ++j, ++cnt) {
-        uint32_t bits[4];
-        const bool partial = (a.mask.key_mask != nullptr || (j + 1) * kTile > w.n_keys) &&
-                             key_bits(a.mask, w.b, a.s.sk, w.n_keys, j, lane, bits);
+        const bool partial = a.mask.key_mask != nullptr || (j + 1) * kTile > w.n_keys;
+        uint32_t bits = 0xffffffffu;  // of this thread's columns
+        if (partial) {
+          uint32_t all[4];
+          key_bits(a.mask, w.b, a.s.sk, w.n_keys, j, lane, all);
+          bits = half == 0 ? (sub == 0 ? all[0] : all[1]) : (sub == 0 ? all[2] : all[3]);
+        }
         ok = warp_wait(&s.s_full[half], cnt & 1, abort_flag, a.sink, 128);
         if (!ok) break;
         tc_fence_after();
-        float p[2][32];
-        tc_ld32(t_s, p[0]);
-        tc_ld32(t_s + 32, p[1]);
+        float p[32];
+        tc_ld32(t_s, p);
         tc_wait_ld();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.p_full[half]);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float2 y = f2_unpack(f2_fma(f2_pack(p[i][e], p[i][e + 1]), c2, nlse2));
-            p[i][e] = ex2_approx(y.x);
-            p[i][e + 1] = ex2_approx(y.y);
-          }
+        for (int e = 0; e < 32; e += 2) {
+          const float2 y = f2_unpack(f2_fma(f2_pack(p[e], p[e + 1]), c2, nlse2));
+          p[e] = ex2_approx(y.x);
+          p[e + 1] = ex2_approx(y.y);
+        }
         ok = warp_wait(&s.dp_full[half], cnt & 1, abort_flag, a.sink, 130);
         if (!ok) break;
         tc_fence_after();
-        float dp[2][32];
-        tc_ld32(t_dp, dp[0]);
-        tc_ld32(t_dp + 32, dp[1]);
+        float dp[32];
+        tc_ld32(t_dp, dp);
         tc_wait_ld();
-        if (partial) {  // S and dP of a masked key may be anything, NaN included
-          const uint32_t b0 = half == 0 ? bits[0] : bits[2], b1 = half == 0 ? bits[1] : bits[3];
+        if (partial && bits != 0xffffffffu) {  // S and dP of a masked key may be anything, NaN included
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
-            p[0][e] = (b0 >> e) & 1u ? p[0][e] : 0.f;
-            p[1][e] = (b1 >> e) & 1u ? p[1][e] : 0.f;
-            dp[0][e] = (b0 >> e) & 1u ? dp[0][e] : 0.f;
-            dp[1][e] = (b1 >> e) & 1u ? dp[1][e] : 0.f;
+            p[e] = (bits >> e) & 1u ? p[e] : 0.f;
+            dp[e] = (bits >> e) & 1u ? dp[e] : 0.f;
           }
-          // ... and its row of K must not reach the last product: this half's 64 rows, two threads each
+          // ... and its row of K must not reach the last product: the 32 rows of this warpgroup's columns
           const int k_at = it1 + 2 * j;
           ok = warp_wait(&s.full[k_at % kRing], (k_at / kRing) & 1, abort_flag, a.sink, 129);
           if (!ok) break;
-          const int key = half * 64 + (r & 63);
-          const uint32_t word = (r & 32) ? b1 : b0;
-          if (r < 64 && !((word >> lane) & 1u)) clear_row<NB>(s.ring[k_at % kRing], key);
+          if (quarter == 0 && !((bits >> lane) & 1u)) clear_row<NB>(s.ring[k_at % kRing], group * 32 + lane);
           fence_proxy_async_smem();
         }
-        if (!w.o) {  // one key tile: delta = sum of P dP over the row's keys, both halves'
+        if (!w.o) {  // one key tile: delta = sum of P dP over the row's keys
           uint64_t acc = 0;
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) acc = f2_fma(f2_pack(p[i][e], p[i][e + 1]), f2_pack(dp[i][e], dp[i][e + 1]), acc);
+          for (int e = 0; e < 32; e += 2) acc = f2_fma(f2_pack(p[e], p[e + 1]), f2_pack(dp[e], dp[e + 1]), acc);
           const float2 v = f2_unpack(acc);
-          float sum = v.x + v.y;
-          if (w.n1 > 0) {
-            s.red[swaps & 1][half][r] = sum;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s.pair[quarter]);
-            ok = warp_wait(&s.pair[quarter], swaps & 1, abort_flag, a.sink, 139);
-            if (!ok) break;
-            sum = s.red[swaps & 1][0][r] + s.red[swaps & 1][1][r];
-            ++swaps;
-          }
-          ndelta = -sum;
+          ok = exchange(-(v.x + v.y), ndelta);
+          if (!ok) break;
         }
-        uint32_t pk[32];
+        uint32_t pk[16];
         const uint64_t nd2 = f2_pack(ndelta * factor, ndelta * factor), factor2 = f2_pack(factor, factor);
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const uint64_t x = f2_pack(dp[i][e], dp[i][e + 1]);
-            const uint64_t d = kHalf ? f2_fma(x, factor2, nd2) : f2_add(x, nd2);
-            const float2 ds = f2_unpack(f2_mul(f2_pack(p[i][e], p[i][e + 1]), d));
-            pk[i * 16 + e / 2] = pack2<T>(ds.x, ds.y);
-          }
+        for (int e = 0; e < 32; e += 2) {
+          const uint64_t x = f2_pack(dp[e], dp[e + 1]);
+          const uint64_t d = kHalf ? f2_fma(x, factor2, nd2) : f2_add(x, nd2);
+          const float2 ds = f2_unpack(f2_mul(f2_pack(p[e], p[e + 1]), d));
+          pk[e / 2] = pack2<T>(ds.x, ds.y);
+        }
         if (cnt > 0) {
           ok = warp_wait(&s.ds_free[half], (cnt - 1) & 1, abort_flag, a.sink, 131);
           if (!ok) break;
           tc_fence_after();
         }
-        tc_st32(t_ds, pk);
+        tc_st16(t_ds, pk);
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -411,34 +408,37 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       }
       if (!ok) break;
       it = it1 + 2 * w.n_t;
-      if (half == 0) {
+      if (group == 0) {
         a.delta[at] = ndelta;
         if constexpr (kHalf) a.peak[at] = peak;
       }
       if (w.n_t > 0) {
+        ++items;
         ok = warp_wait(&s.acc_done, (items - 1) & 1, abort_flag, a.sink, 132);
         if (!ok) break;
         tc_fence_after();
       }
-      const int pos = w.qt * pos_per_tile + quarter * 32 / a.s.gp;
-      const float mul = a.scale / factor;
-      for (int c = half * 32; c < a.s.d; c += 64) {
-        float o[32];
-        tc_ld32(t_dq + c, o);
-        tc_wait_ld();
+      if (half == 0) {  // its next dS is what the next item's first product waits for
+        const int pos = w.qt * pos_per_tile + quarter * 32 / a.s.gp;
+        const float mul = a.scale / factor;
+        for (int c = sub * 32; c < a.s.d; c += 64) {
+          float o[32];
+          tc_ld32(t_dq + c, o);
+          tc_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = w.n_t == 0 ? 0.f : o[e] * mul;
-        store_block<T>(&map_dq, stage, o, lane, c, w.hb * a.s.gp, pos, w.b, pos < a.s.sq);
+          for (int e = 0; e < 32; ++e) o[e] = w.n_t == 0 ? 0.f : o[e] * mul;
+          store_block<T>(&map_dq, s.out[warp], o, lane, c, w.hb * a.s.gp, pos, w.b, pos < a.s.sq);
+        }
+        tc_fence_before();
       }
-      tc_fence_before();
     }
-    if (lane == 0) bulk_wait_all();
+    if (half == 0 && lane == 0) bulk_wait_all();
     __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 9) tmem_free<512>(tmem);
+  if (warp == 17) tmem_free<512>(tmem);
 }
 
 // ------------------------------------------------------------------ dK and dV
@@ -456,7 +456,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort_flag = &s.abort_flag;
   if (threadIdx.x == 0) bwd_init<NB>(s);
-  if (warp == 9) tmem_alloc<512>(&s.tmem_base);
+  if (warp == 17) tmem_alloc<512>(&s.tmem_base);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -485,7 +485,9 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     return w;
   };
 
-  if (warp == 8) {
+  if (warp >= 16) {
+   reg_give<64>();
+   if (warp == 16) {
     int it = 0, cnt = 0;
     bool ok = true;
     for (int item = blockIdx.x; item < a.items && ok; item += gridDim.x) {
@@ -520,7 +522,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       ++cnt;
     }
     if (!ok) settle();
-  } else if (warp == 9) {
+   } else if (warp == 17) {
     const int ksteps = a.s.dn / 16;
     const uint32_t id_s = attn_idesc(kFmt, 64, false), id_o = attn_idesc(kFmt, a.s.dn, true);
     const uint64_t res = desc_k(smem_u32(s.res[0])), ring = desc_k(smem_u32(s.ring[0])), ring_mn = desc_mn<>(smem_u32(s.ring[0]));
@@ -556,7 +558,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         // acc += A(i) of half h times the rows of that half of the tile in ring position `at`
         auto issue_acc = [&](uint32_t acc, uint32_t src, int at, int i, int h) {
           tc_fence_after();
-          issue_tn<4>(acc, src + h * 64, 0, ring_mn + (at % kRing) * kStep + h * kHalfRows, 4, id_o, (i > 0 || h > 0) ? 1u : 0u);
+          issue_tn<4, 2>(acc, src + h * 64, 32, ring_mn + (at % kRing) * kStep + h * kHalfRows, 4, id_o, (i > 0 || h > 0) ? 1u : 0u);
         };
         wait(&s.res_full, static_cast<uint32_t>(cnt), 144);
         for (int h = 0; h < 2; ++h)
@@ -595,11 +597,12 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       ++cnt;
     }
     __syncwarp();
+   }
   } else {
-    const int half = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    reg_take<104>();
+    const int half = warp >> 3, sub = (warp >> 2) & 1, group = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t t_s = tmem + lanes + half * 64, t_dp = t_s + 128, t_dv = tmem + lanes + 256, t_dk = tmem + lanes + 384;
-    uint8_t* stage = s.out[warp];
+    const uint32_t t_s = tmem + lanes + group * 32, t_dp = t_s + 128, t_dv = tmem + lanes + 256, t_dk = tmem + lanes + 384;
     uint32_t cnt = 0, done = 0;
     int it = 0;
     bool ok = true;
@@ -611,16 +614,16 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       if (w.n_i > 0) {
         uint32_t bits[4];
         key_bits(a.mask, w.b, a.s.sk, w.n_keys, w.kt, lane, bits);
-        mine = (bits[quarter] >> lane) & 1u;
+        mine = ((quarter < 2 ? (quarter == 0 ? bits[0] : bits[1]) : (quarter == 2 ? bits[2] : bits[3])) >> lane) & 1u;
       }
       float factor = 1.f;  // fp16: on dS
       if constexpr (kHalf) {
         if (w.n_i > 0) {
           float top = 0.f;
-          for (int i = 0; i < w.n_i; ++i) {
-            const int sub = (w.i0 + i) / a.s.qtiles, qt = (w.i0 + i) - sub * a.s.qtiles;
+          for (int i = 0; i < a.steps; ++i) {
+            const int sub_block = i / a.s.qtiles, qt = i - sub_block * a.s.qtiles;
             const float4 v = __ldg(reinterpret_cast<const float4*>(
-                a.peak + (static_cast<long long>(w.b) * a.s.hb + w.h * group_blocks + sub) * a.s.rows_pad + qt * kTile) + lane);
+                a.peak + (static_cast<long long>(w.b) * a.s.hb + w.h * group_blocks + sub_block) * a.s.rows_pad + qt * kTile) + lane);
             top = max3(max3(top, v.x, v.y), v.z, v.w);
           }
 #pragma unroll
@@ -630,39 +633,36 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       }
       const float p_up = kHalf ? exp2f(a.p_shift) : 1.f;
       const uint64_t c2 = f2_pack(a.c, a.c), shift2 = f2_pack(a.p_shift, a.p_shift);
-      const uint64_t f2 = f2_pack(factor / p_up, factor / p_up);
-      const bool any = __any_sync(0xffffffffu, mine);  // rows of a warp without keys stay as they are: zeros are written
+      const uint64_t fac2 = f2_pack(factor / p_up, factor / p_up);
+      const bool any = __any_sync(0xffffffffu, mine);  // a warp without keys leaves its rows as they are: zeros are written
       for (int i = 0; i < w.n_i; ++i, ++cnt) {
         const int qa = it0 + 2 * i;
         ok = warp_wait(&s.full[qa % kRing], (qa / kRing) & 1, abort_flag, a.sink, 149);  // the statistics have landed
         if (!ok) break;
-        const ulonglong2* st_l = reinterpret_cast<const ulonglong2*>(s.stat[(qa % kRing) / 2][0]) + half * 16;
-        const ulonglong2* st_d = reinterpret_cast<const ulonglong2*>(s.stat[(qa % kRing) / 2][1]) + half * 16;
+        const ulonglong2* st_l = reinterpret_cast<const ulonglong2*>(s.stat[(qa % kRing) / 2][0]) + group * 8;
+        const ulonglong2* st_d = reinterpret_cast<const ulonglong2*>(s.stat[(qa % kRing) / 2][1]) + group * 8;
         ok = warp_wait(&s.s_full[half], cnt & 1, abort_flag, a.sink, 150);
         if (!ok) break;
         tc_fence_after();
-        float p[2][32];
-        uint32_t pk[32];
+        float p[32];
+        uint32_t pk[16];
         if (any) {
-          tc_ld32(t_s, p[0]);
-          tc_ld32(t_s + 32, p[1]);
+          tc_ld32(t_s, p);
           tc_wait_ld();
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              const ulonglong2 l4 = st_l[h * 8 + e / 4];
-              const uint64_t la = kHalf ? f2_add(l4.x, shift2) : l4.x, lb = kHalf ? f2_add(l4.y, shift2) : l4.y;
-              const float2 ya = f2_unpack(f2_fma(f2_pack(p[h][e], p[h][e + 1]), c2, la));
-              const float2 yb = f2_unpack(f2_fma(f2_pack(p[h][e + 2], p[h][e + 3]), c2, lb));
-              p[h][e] = ex2_approx(ya.x);
-              p[h][e + 1] = ex2_approx(ya.y);
-              p[h][e + 2] = ex2_approx(yb.x);
-              p[h][e + 3] = ex2_approx(yb.y);
-              pk[h * 16 + e / 2] = pack2<T>(p[h][e], p[h][e + 1]);
-              pk[h * 16 + e / 2 + 1] = pack2<T>(p[h][e + 2], p[h][e + 3]);
-            }
-          tc_st32(t_s, pk);
+          for (int e = 0; e < 32; e += 4) {
+            const ulonglong2 l4 = st_l[e / 4];
+            const uint64_t la = kHalf ? f2_add(l4.x, shift2) : l4.x, lb = kHalf ? f2_add(l4.y, shift2) : l4.y;
+            const float2 ya = f2_unpack(f2_fma(f2_pack(p[e], p[e + 1]), c2, la));
+            const float2 yb = f2_unpack(f2_fma(f2_pack(p[e + 2], p[e + 3]), c2, lb));
+            p[e] = ex2_approx(ya.x);
+            p[e + 1] = ex2_approx(ya.y);
+            p[e + 2] = ex2_approx(yb.x);
+            p[e + 3] = ex2_approx(yb.y);
+            pk[e / 2] = pack2<T>(p[e], p[e + 1]);
+            pk[e / 2 + 1] = pack2<T>(p[e + 2], p[e + 3]);
+          }
+          tc_st16(t_s, pk);
           tc_wait_st();
         }
         tc_fence_before();
@@ -672,26 +672,23 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         if (!ok) break;
         tc_fence_after();
         if (any) {
-          float dp[2][32];
-          tc_ld32(t_dp, dp[0]);
-          tc_ld32(t_dp + 32, dp[1]);
+          float dp[32];
+          tc_ld32(t_dp, dp);
           tc_wait_ld();
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              const ulonglong2 d4 = st_d[h * 8 + e / 4];
-              uint64_t da = f2_add(f2_pack(dp[h][e], dp[h][e + 1]), d4.x), db = f2_add(f2_pack(dp[h][e + 2], dp[h][e + 3]), d4.y);
-              if constexpr (kHalf) {
-                da = f2_mul(da, f2);
-                db = f2_mul(db, f2);
-              }
-              const float2 sa = f2_unpack(f2_mul(f2_pack(p[h][e], p[h][e + 1]), da));
-              const float2 sb = f2_unpack(f2_mul(f2_pack(p[h][e + 2], p[h][e + 3]), db));
-              pk[h * 16 + e / 2] = pack2<T>(sa.x, sa.y);
-              pk[h * 16 + e / 2 + 1] = pack2<T>(sb.x, sb.y);
+          for (int e = 0; e < 32; e += 4) {
+            const ulonglong2 d4 = st_d[e / 4];
+            uint64_t da = f2_add(f2_pack(dp[e], dp[e + 1]), d4.x), db = f2_add(f2_pack(dp[e + 2], dp[e + 3]), d4.y);
+            if constexpr (kHalf) {
+              da = f2_mul(da, fac2);
+              db = f2_mul(db, fac2);
             }
-          tc_st32(t_dp, pk);
+            const float2 sa = f2_unpack(f2_mul(f2_pack(p[e], p[e + 1]), da));
+            const float2 sb = f2_unpack(f2_mul(f2_pack(p[e + 2], p[e + 3]), db));
+            pk[e / 2] = pack2<T>(sa.x, sa.y);
+            pk[e / 2 + 1] = pack2<T>(sb.x, sb.y);
+          }
+          tc_st16(t_dp, pk);
           tc_wait_st();
         }
         tc_fence_before();
@@ -699,18 +696,19 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         if (lane == 0) mbar_arrive(&s.ds_full[half]);
       }
       if (!ok) break;
+      if (half == 1) continue;
       if (w.n_i > 0) {
         ok = warp_wait(&s.acc_done, done & 1, abort_flag, a.sink, 152);
         if (!ok) break;
         ++done;
         tc_fence_after();
       }
-      // dV, then dK, 32 columns at a time, the two halves taking turns
+      // dV, then dK, 32 columns at a time; this half's next P and dS are what the next item's first products wait for
       const int key = w.kt * kTile + r;
       for (int which = 0; which < 2; ++which) {
         const uint32_t src = which == 0 ? t_dv : t_dk;
         const float mul = which == 0 ? 1.f / p_up : a.scale / factor;
-        for (int c = half * 32; c < a.s.d; c += 64) {
+        for (int c = sub * 32; c < a.s.d; c += 64) {
           float o[32];
           tc_ld32(src + c, o);
           tc_wait_ld();
@@ -727,19 +725,19 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             }
           } else {
             const int k0 = w.kt * kTile + quarter * 32;
-            store_block<T>(which == 0 ? &map_dv : &map_dk, stage, o, lane, c, w.h, k0, w.b, k0 < a.s.sk);
+            store_block<T>(which == 0 ? &map_dv : &map_dk, s.out[warp], o, lane, c, w.h, k0, w.b, k0 < a.s.sk);
           }
         }
       }
       tc_fence_before();
     }
-    if (lane == 0) bulk_wait_all();
+    if (half == 0 && lane == 0) bulk_wait_all();
     __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 9) tmem_free<512>(tmem);
+  if (warp == 17) tmem_free<512>(tmem);
 }
 
 // adds the partial dK and dV of the query ranges, in their order

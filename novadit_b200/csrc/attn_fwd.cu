@@ -196,7 +196,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
               if (ok) ok = mbar_wait(&s.p_full[t], (base[t] + j) & 1, abort_flag, a.sink, 105);
               if (!ok) break;
               tc_fence_after();
-              issue_tn<kCh>(tm_o + t * a.s.dn, tm_p + t * (KT / 2), 32, v_desc + (v_at % kKv) * (kKvBytes >> 4), steps, id_o,
+              issue_tn<kCh, kCh>(tm_o + t * a.s.dn, tm_p + t * (KT / 2), 0, v_desc + (v_at % kKv) * (kKvBytes >> 4), steps, id_o,
                             j > 0 ? 1u : 0u);
               mma_commit(&s.o_done[t]);
               if (t == nt - 1) mma_commit(&s.kv_empty[v_at % kKv]);
