@@ -78,12 +78,6 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
       ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
-__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* src, int c0, int c1, int c2, int c3) {
-  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
-               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-               : "memory");
-}
-
 // a tile of NB 64-column blocks of ROWS rows
 template <int NB, int ROWS = kTile>
 __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int head, int pos, int b) {
@@ -180,6 +174,19 @@ __device__ __forceinline__ int key_count(const AttnMask& m, int b, int sk, int l
   return 0;
 }
 
+__device__ __forceinline__ void fill_lens(int* lens, const AttnMask& m, int batch, int sk, int warp, int warps, int lane) {
+  for (int b = warp; b < batch; b += warps) {
+    const int n = key_count(m, b, sk, lane);
+    if (lane == 0) lens[b] = n;
+  }
+}
+
+// The key mask of keys at .. at + 31 that lie below n_keys; called by whole warps.
+__device__ __forceinline__ uint32_t key_word(const AttnMask& m, int b, int sk, int n_keys, int at, int lane) {
+  const bool on = at + lane < n_keys && __ldg(m.key_mask + static_cast<long long>(b) * sk + at + lane) != 0;
+  return __ballot_sync(0xffffffffu, on);
+}
+
 // Which of the KT keys of tile `kt` take part, 32 per word; called by whole warps. True: some do not.
 template <int KT = kTile>
 __device__ __forceinline__ bool key_bits(const AttnMask& m, int b, int sk, int n_keys, int kt, int lane, uint32_t (&bits)[4]) {
@@ -191,10 +198,7 @@ __device__ __forceinline__ bool key_bits(const AttnMask& m, int b, int sk, int n
     const int left = end - at;
     const uint32_t all = KT - i * 32 >= 32 ? 0xffffffffu : (KT <= i * 32 ? 0u : (1u << (KT & 31)) - 1u);
     bits[i] = left >= 32 ? 0xffffffffu : (left <= 0 ? 0u : (1u << left) - 1u);
-    if (m.key_mask != nullptr) {
-      const bool on = at + lane < end && __ldg(m.key_mask + static_cast<long long>(b) * sk + at + lane) != 0;
-      bits[i] = __ballot_sync(0xffffffffu, on);
-    }
+    if (m.key_mask != nullptr) bits[i] = key_word(m, b, sk, end, at, lane);
     partial |= bits[i] != all;
   }
   return partial;
@@ -232,28 +236,30 @@ template <int NB, int ROWS = kTile> __device__ __forceinline__ void clear_row(ui
     for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(tile + i * ROWS * 128 + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
 }
 
-// One warp's 32 rows x 32 columns of 16-bit values (lane = row) through a 2 KB staging block to the copy engine.
-template <typename T>
-__device__ __forceinline__ void store_block(const CUtensorMap* map, uint8_t* stage, const float (&v)[32], int lane, int col,
-                                            int head, int pos, int b, bool inside) {
-  if (lane == 0) bulk_wait_read_all();  // the previous block has left the staging memory
-  __syncwarp();
+// One warp's 32 rows x 32 columns of 16-bit values (lane = row) in a 2 KB staging block, 64-byte swizzle, for the copy
+// engine. A thread that writes its own row to global memory costs one line per lane and instruction (3900 cycles for the
+// two tiles of an item at D = 72); a block that is waited for before the next is staged costs about as much. So a
+// warp stages all its blocks, hands them over and looks at them again only when it needs the memory for the next item.
+constexpr int kStageBytes = 2048;
+template <typename T> __device__ __forceinline__ void stage_block(uint8_t* stage, const float (&v)[32], int lane) {
   const int sw = (lane >> 1) & 3;
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    uint4 pk;
-    pk.x = pack2<T>(v[c * 8 + 0], v[c * 8 + 1]);
-    pk.y = pack2<T>(v[c * 8 + 2], v[c * 8 + 3]);
-    pk.z = pack2<T>(v[c * 8 + 4], v[c * 8 + 5]);
-    pk.w = pack2<T>(v[c * 8 + 6], v[c * 8 + 7]);
-    *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ sw) << 4)) = pk;
-  }
-  fence_proxy_async_smem();
-  __syncwarp();
-  if (lane == 0 && inside) {
-    tma_store_4d(map, stage, col, head, pos, b);
-    bulk_commit();
-  }
+  for (int c = 0; c < 4; ++c)
+    *reinterpret_cast<uint4*>(stage + lane * 64 + ((c ^ sw) << 4)) =
+        make_uint4(pack2<T>(v[c * 8 + 0], v[c * 8 + 1]), pack2<T>(v[c * 8 + 2], v[c * 8 + 3]),
+                   pack2<T>(v[c * 8 + 4], v[c * 8 + 5]), pack2<T>(v[c * 8 + 6], v[c * 8 + 7]));
+}
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
+}
+
+// Key counts of all samples, worked out once by all warps of a CTA where they fit: every role of every item asks for one,
+// and a dependent load from global memory each time is most of a short item's start.
+constexpr int kLens = 256;
+__device__ __forceinline__ bool lens_cached(const AttnMask& m, int batch, int sk) {
+  return batch <= kLens && (m.key_mask == nullptr || static_cast<long long>(batch) * sk <= 65536);
 }
 
 // let copies already issued land in shared memory before the CTA may exit (after an expired wait)

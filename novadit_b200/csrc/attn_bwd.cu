@@ -48,7 +48,10 @@ template <int NB> struct __align__(1024) BwdSmem {
   static constexpr int kRing = NB == 1 ? 8 : 4;
   uint8_t res[2][NB * kBlkBytes];        // dQ: Q, dO; dK/dV: K, V
   uint8_t ring[kRing][NB * kBlkBytes];   // dQ: K, V, K, V, ...; dK/dV: Q, dO, ...
-  uint8_t out[8][2048];                  // staging of the first half's warps, which write the results
+  // staging of the first half's warps, which write the results: block c of 32 rows holds columns 32 c .., the fourth goes
+  // where the second was
+  uint8_t out[4][(NB == 1 ? 2 : 3) * kStageBytes];
+  int lens[kLens];
   alignas(16) float stat[kRing / 2][2][kTile];  // dK/dV: log-sum-exp and delta of the query tile
   uint64_t res_full, res_empty;
   uint64_t full[kRing], empty[kRing];
@@ -102,6 +105,24 @@ template <typename T> __device__ __forceinline__ float peak8(const uint4& v, flo
   return top;
 }
 
+// 32 rows x 32 columns from `c` on, through the block of their own and to the copy engine
+template <typename T>
+__device__ __forceinline__ void put_block(const CUtensorMap* map, uint8_t* out, const float (&v)[32], int lane, int c, int head,
+                                          int pos, int b, bool inside) {
+  if (c == 96) {
+    if (lane == 0) bulk_wait_read_all();
+    __syncwarp();
+  }
+  uint8_t* stage = out + (c == 96 ? 1 : c / 32) * kStageBytes;
+  stage_block<T>(stage, v, lane);
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0 && inside) {
+    tma_store_4d(map, stage, c, head, pos, b);
+    bulk_commit();
+  }
+}
+
 // ------------------------------------------------------------------ dQ
 // TMEM columns: S 0, dP 128, dS 256 (32 columns of 16-bit pairs per half), dQ 384
 template <int NB, typename T>
@@ -118,12 +139,14 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
   volatile int* abort_flag = &s.abort_flag;
   if (threadIdx.x == 0) bwd_init<NB>(s);
   if (warp == 17) tmem_alloc<512>(&s.tmem_base);
+  griddep_launch_dependents();
+  griddep_wait();
+  const bool cached = lens_cached(a.mask, a.s.batch, a.s.sk);
+  if (cached) fill_lens(s.lens, a.mask, a.s.batch, a.s.sk, warp, kBwdThreads / 32, lane);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s.tmem_base;
-  griddep_launch_dependents();
-  griddep_wait();
 
   const int group_blocks = a.s.hb / a.s.hkv;
   const int pos_per_tile = kTile / a.s.gp;
@@ -139,7 +162,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     const int r = item / a.s.qtiles;
     w.hb = r % a.s.hb;
     w.b = r / a.s.hb;
-    w.n_keys = key_count(a.mask, w.b, a.s.sk, lane);
+    w.n_keys = cached ? s.lens[w.b] : key_count(a.mask, w.b, a.s.sk, lane);
     w.n_t = (w.n_keys + kTile - 1) / kTile;
     w.n1 = (w.n_keys + 63) / kTile;
     w.o = w.n_t > 1 ? 1 : 0;
@@ -337,13 +360,9 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       const int mine = half == 0 ? w.n_t : w.n1;
       const uint64_t c2 = f2_pack(a.c, a.c), nlse2 = f2_pack(nlse, nlse);
       for (int j = 0; j < mine; ++j, ++cnt) {
-        const bool partial = a.mask.key_mask != nullptr || (j + 1) * kTile > w.n_keys;
-        uint32_t bits = 0xffffffffu;  // of this thread's columns
-        if (partial) {
-          uint32_t all[4];
-          key_bits(a.mask, w.b, a.s.sk, w.n_keys, j, lane, all);
-          bits = half == 0 ? (sub == 0 ? all[0] : all[1]) : (sub == 0 ? all[2] : all[3]);
-        }
+        const int col = j * kTile + group * 32, left = w.n_keys - col;  // this thread's columns
+        uint32_t bits = left >= 32 ? 0xffffffffu : (left <= 0 ? 0u : (1u << left) - 1u);
+        if (a.mask.key_mask != nullptr) bits = key_word(a.mask, w.b, a.s.sk, w.n_keys, col, lane);
         ok = warp_wait(&s.s_full[half], cnt & 1, abort_flag, a.sink, 128);
         if (!ok) break;
         tc_fence_after();
@@ -365,7 +384,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         float dp[32];
         tc_ld32(t_dp, dp);
         tc_wait_ld();
-        if (partial && bits != 0xffffffffu) {  // S and dP of a masked key may be anything, NaN included
+        if (bits != 0xffffffffu) {  // S and dP of a masked key may be anything, NaN included
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             p[e] = (bits >> e) & 1u ? p[e] : 0.f;
@@ -419,20 +438,22 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         tc_fence_after();
       }
       if (half == 0) {  // its next dS is what the next item's first product waits for
-        const int pos = w.qt * pos_per_tile + quarter * 32 / a.s.gp;
         const float mul = a.scale / factor;
+        const int pos = w.qt * pos_per_tile + quarter * 32 / a.s.gp;
+        if (lane == 0) bulk_wait_read_all();  // the blocks of the item before have left
+        __syncwarp();
         for (int c = sub * 32; c < a.s.d; c += 64) {
           float o[32];
           tc_ld32(t_dq + c, o);
           tc_wait_ld();
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = w.n_t == 0 ? 0.f : o[e] * mul;
-          store_block<T>(&map_dq, s.out[warp], o, lane, c, w.hb * a.s.gp, pos, w.b, pos < a.s.sq);
+          put_block<T>(&map_dq, s.out[quarter], o, lane, c, w.hb * a.s.gp, pos, w.b, pos < a.s.sq);
         }
         tc_fence_before();
       }
     }
-    if (half == 0 && lane == 0) bulk_wait_all();
+    if (half == 0 && lane == 0) bulk_wait_all();  // this warp's blocks are written before the CTA may exit
     __syncwarp();
   }
   tc_fence_before();
@@ -457,12 +478,14 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
   volatile int* abort_flag = &s.abort_flag;
   if (threadIdx.x == 0) bwd_init<NB>(s);
   if (warp == 17) tmem_alloc<512>(&s.tmem_base);
+  griddep_launch_dependents();
+  griddep_wait();
+  const bool cached = lens_cached(a.mask, a.s.batch, a.s.sk);
+  if (cached) fill_lens(s.lens, a.mask, a.s.batch, a.s.sk, warp, kBwdThreads / 32, lane);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s.tmem_base;
-  griddep_launch_dependents();
-  griddep_wait();
 
   const int group_blocks = a.s.hb / a.s.hkv;
   const int pos_per_tile = kTile / a.s.gp;
@@ -478,7 +501,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     r /= a.s.ktiles;
     w.h = r % a.s.hkv;
     w.b = r / a.s.hkv;
-    w.n_keys = key_count(a.mask, w.b, a.s.sk, lane);
+    w.n_keys = cached ? s.lens[w.b] : key_count(a.mask, w.b, a.s.sk, lane);
     w.i0 = w.split * a.steps_per_split;
     w.n_i = a.steps - w.i0 < a.steps_per_split ? a.steps - w.i0 : a.steps_per_split;
     if (w.kt * kTile >= w.n_keys || w.n_i < 0) w.n_i = 0;
@@ -706,6 +729,8 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       // dV, then dK, 32 columns at a time; this half's next P and dS are what the next item's first products wait for
       const int key = w.kt * kTile + r;
       for (int which = 0; which < 2; ++which) {
+        if (lane == 0) bulk_wait_read_all();  // the blocks before have left
+        __syncwarp();
         const uint32_t src = which == 0 ? t_dv : t_dk;
         const float mul = which == 0 ? 1.f / p_up : a.scale / factor;
         for (int c = sub * 32; c < a.s.d; c += 64) {
@@ -725,13 +750,13 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             }
           } else {
             const int k0 = w.kt * kTile + quarter * 32;
-            store_block<T>(which == 0 ? &map_dv : &map_dk, s.out[warp], o, lane, c, w.h, k0, w.b, k0 < a.s.sk);
+            put_block<T>(which == 0 ? &map_dv : &map_dk, s.out[quarter], o, lane, c, w.h, k0, w.b, k0 < a.s.sk);
           }
         }
       }
       tc_fence_before();
     }
-    if (half == 0 && lane == 0) bulk_wait_all();
+    if (half == 0 && lane == 0) bulk_wait_all();  // this warp's blocks are written before the CTA may exit
     __syncwarp();
   }
   tc_fence_before();

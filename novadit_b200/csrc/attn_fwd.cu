@@ -38,7 +38,8 @@ template <int NB, int KT> struct __align__(1024) FwdSmem {
   static constexpr int kKv = NB == 1 ? 8 : 4;  // key / value tiles in flight
   uint8_t q[2][NB * kBlkBytes];
   uint8_t kv[kKv][NB * KT * 128];
-  uint8_t out[8][2048];
+  uint8_t out[8][(NB == 1 ? 2 : KT == 112 ? 3 : 4) * kStageBytes];  // every warp's rows
+  int lens[kLens];
   uint64_t q_full, q_empty;
   uint64_t kv_full[kKv], kv_empty[kKv];
   uint64_t s_full[2], s_free[2], p_full[2], o_done[2];
@@ -63,7 +64,7 @@ struct FwdItem {
   bool two;                                 // the pair's second tile has rows
 };
 
-template <int KT> __device__ __forceinline__ FwdItem fwd_item(const FwdArgs& a, int item, int lane) {
+template <int KT> __device__ __forceinline__ FwdItem fwd_item(const FwdArgs& a, const int* lens, int item, int lane) {
   FwdItem w;
   w.split = item % a.splits;
   int r = item / a.splits;
@@ -72,7 +73,7 @@ template <int KT> __device__ __forceinline__ FwdItem fwd_item(const FwdArgs& a, 
   w.hb = r % a.s.hb;
   w.b = r / a.s.hb;
   w.two = 2 * w.pair + 1 < a.s.qtiles;
-  w.n_keys = key_count(a.mask, w.b, a.s.sk, lane);
+  w.n_keys = lens != nullptr ? lens[w.b] : key_count(a.mask, w.b, a.s.sk, lane);
   const int all = (w.n_keys + KT - 1) / KT;
   w.t0 = w.split * a.tiles_per_split;
   const int left = all - w.t0;
@@ -110,12 +111,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 9) tmem_alloc<512>(&s.tmem_base);
+  griddep_launch_dependents();
+  griddep_wait();
+  const int* lens = lens_cached(a.mask, a.s.batch, a.s.sk) ? s.lens : nullptr;
+  if (lens != nullptr) fill_lens(s.lens, a.mask, a.s.batch, a.s.sk, warp, kFwdThreads / 32, lane);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s.tmem_base;
-  griddep_launch_dependents();
-  griddep_wait();
 
   const int group_blocks = a.s.hb / a.s.hkv;  // head blocks per key head
   const int pos_per_tile = kTile / a.s.gp;
@@ -129,7 +132,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     int it = 0, q_cnt = 0;
     bool ok = true;
     for (int item = blockIdx.x; item < a.items && ok; item += gridDim.x) {
-      const FwdItem w = fwd_item<KT>(a, item, lane);
+      const FwdItem w = fwd_item<KT>(a, lens, item, lane);
       if (w.n_t == 0) continue;
       if (lane == 0) {
         const int kvh = w.hb / group_blocks;
@@ -161,7 +164,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     uint32_t base[2] = {0, 0};  // key tiles of the items before, per query tile
     bool ok = true;
     for (int item = blockIdx.x; item < a.items && ok; item += gridDim.x) {
-      const FwdItem w = fwd_item<KT>(a, item, lane);
+      const FwdItem w = fwd_item<KT>(a, lens, item, lane);
       if (w.n_t == 0) continue;
       const int nt = w.two ? 2 : 1;
       if (elect_one()) {
@@ -218,12 +221,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const int t = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t ts = tmem + lanes + t * KT, tp = tm_p + lanes + t * (KT / 2), to = tm_o + lanes + t * a.s.dn;
-    uint8_t* stage = s.out[warp];
     uint32_t cnt = 0;  // key tiles so far
     int it = 0;
     bool ok = true;
     for (int item = blockIdx.x; item < a.items && ok; item += gridDim.x) {
-      const FwdItem w = fwd_item<KT>(a, item, lane);
+      const FwdItem w = fwd_item<KT>(a, lens, item, lane);
       const int it0 = it;
       it += 2 * w.n_t;
       if (t == 1 && !w.two) continue;
@@ -314,26 +316,38 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         } else {
           const int left = w.n_keys - (w.t0 + j) * KT;
           const int n_ch = left >= KT ? kCh : (left + 15) >> 4;  // the others were not even computed
-          uint32_t bits[4];
-          const bool partial = key_bits<KT>(a.mask, w.b, a.s.sk, w.n_keys, w.t0 + j, lane, bits);
 #pragma unroll
           for (int i = 0; i < kCh; ++i) tc_ld16(ts + i * 16, x[i]);
           tc_wait_ld();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&s.s_free[t]);
-          if (partial) {
+          bool clear = false;  // this thread's key of the tile takes no part
+          if (a.mask.key_mask != nullptr) {
+            uint32_t bits[4];
+            key_bits<KT>(a.mask, w.b, a.s.sk, w.n_keys, w.t0 + j, lane, bits);
 #pragma unroll
             for (int i = 0; i < kCh; ++i)
 #pragma unroll
               for (int e = 0; e < 16; ++e) x[i][e] = (bits[i >> 1] >> ((i & 1) * 16 + e)) & 1u ? x[i][e] : -INFINITY;
-            if (t == 0) {  // O(j) of tile 1 is issued after that of tile 0: one warpgroup's clearing serves both
-              const int v_at = it0 + 2 * j + 1;
-              ok = warp_wait(&s.kv_full[v_at % kKv], (v_at / kKv) & 1, abort_flag, a.sink, 108);
-              if (!ok) break;
-              if (r < KT && !((bits[quarter] >> lane) & 1u)) clear_row<NB, KT>(s.kv[v_at % kKv], r);
-              fence_proxy_async_smem();
+            clear = r < KT && !((bits[quarter] >> lane) & 1u);
+          } else if (left < KT) {  // the end of the keys: one chunk is cut, those behind it are not looked at
+#pragma unroll
+            for (int i = 0; i < kCh; ++i) {
+              if (left - i * 16 < 16) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[i][e] = e < left - i * 16 ? x[i][e] : -INFINITY;
+              }
             }
+            clear = r < n_ch * 16 && r >= left;
+          }
+          // O(j) of tile 1 is issued after that of tile 0: one warpgroup's clearing serves both
+          if (t == 0 && __any_sync(0xffffffffu, clear)) {
+            const int v_at = it0 + 2 * j + 1;
+            ok = warp_wait(&s.kv_full[v_at % kKv], (v_at / kKv) & 1, abort_flag, a.sink, 108);
+            if (!ok) break;
+            if (clear) clear_row<NB, KT>(s.kv[v_at % kKv], r);
+            fence_proxy_async_smem();
           }
           if (j > 0) {
             ok = warp_wait(&s.o_done[t], (cnt - 1) & 1, abort_flag, a.sink, 111);
@@ -380,7 +394,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         if (a.lse != nullptr)  // -inf where there is nothing: 2^(s - inf) = 0 in the backward pass
           a.lse[head_row * a.s.rows_pad + row] = (l == 0.f || row >= a.s.rows) ? -INFINITY : -(m * a.c + log2f(l));
         const int pos = (2 * w.pair + t) * pos_per_tile + quarter * 32 / a.s.gp;
-        for (int c = 0; c < a.s.d; c += 32) {
+        if (lane == 0) bulk_wait_read_all();  // the blocks of the item before have left
+        __syncwarp();
+#pragma unroll
+        for (int c = 0; c < static_cast<int>(sizeof(s.out[0])) / kStageBytes * 32; c += 32) {
+          if (c >= a.s.d) break;
           float o[2][16];
           tc_ld16(to + c, o[0]);
           if (c + 16 < a.s.dn) tc_ld16(to + c + 16, o[1]);  // (columns behind dn are clipped when the block is stored)
@@ -388,12 +406,18 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           float v[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = l == 0.f ? 0.f : o[e >> 4][e & 15] * inv;
-          store_block<T>(&map_o, stage, v, lane, c, w.hb * a.s.gp, pos, w.b, pos < a.s.sq);
+          stage_block<T>(s.out[warp] + c / 32 * kStageBytes, v, lane);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && pos < a.s.sq) {
+          for (int c = 0; c < a.s.d; c += 32) tma_store_4d(&map_o, s.out[warp] + c / 32 * kStageBytes, c, w.hb * a.s.gp, pos, w.b);
+          bulk_commit();
         }
       }
       tc_fence_before();  // these reads of O come before the next item's products
     }
-    if (lane == 0) bulk_wait_all();  // this warp's output blocks are written before the CTA may exit
+    if (lane == 0) bulk_wait_all();  // this warp's blocks are written before the CTA may exit
     __syncwarp();
   }
   tc_fence_before();
