@@ -44,6 +44,7 @@ CU_SOURCES = [
     "rotary.cu",
     "attn_fwd.cu",
     "attn_bwd.cu",
+    "attn_few.cu",
     "quant.cu",
     "fc1.cu",
     "noalloc.cu",

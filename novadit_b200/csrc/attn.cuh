@@ -42,7 +42,12 @@ inline AttnShape attn_shape(int64_t b, int64_t sq, int64_t sk, int64_t hq, int64
   return s;
 }
 
-int attn_launch(const void* fn, int grid, int threads, size_t smem, void** params, cudaStream_t st);
+int attn_launch(const void* fn, dim3 grid, int threads, size_t smem, void** params, cudaStream_t st);
+// few query rows per key head (attn_few.cu)
+bool attn_few_takes(const AttnShape& s);
+size_t attn_few_ws(const AttnShape& s);
+int attn_few(int dtype, const void* q, const void* k, const void* v, void* out, float* lse, const AttnMask& mask,
+             const AttnShape& s, const int64_t* strides, float c, void* ws, cudaStream_t st);
 
 inline int attn_check(int dtype, int64_t b, int64_t sq, int64_t sk, int64_t hq, int64_t hkv, int64_t d, float scale) {
   if (b < 0 || sq < 0 || sk < 0 || hq <= 0 || hkv <= 0 || d <= 0 || hq % hkv != 0) return ND_ERR_BAD_ARG;

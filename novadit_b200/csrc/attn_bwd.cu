@@ -887,17 +887,17 @@ int nd_attn_bwd(int dtype, const void* dout, const void* q, const void* k, const
                        : (bf ? (const void*)attn_dkv_kernel<2, __nv_bfloat16> : (const void*)attn_dkv_kernel<2, __half>);
   a.items = static_cast<int>(q_items);
   void* p1[] = {&mq, &mdo, &mo, &mk, &mv, &mdq, &a};
-  int e = attn_launch(f1, a.items < sms ? a.items : sms, kBwdThreads, smem, p1, st);
+  int e = attn_launch(f1, dim3(a.items < sms ? a.items : sms), kBwdThreads, smem, p1, st);
   if (e != ND_OK) return e;
   a.items = static_cast<int>(k_items);
   void* p2[] = {&mq, &mdo, &mk, &mv, &mdk, &mdv, &a};
-  e = attn_launch(f2, a.items < sms ? a.items : sms, kBwdThreads, smem, p2, st);
+  e = attn_launch(f2, dim3(a.items < sms ? a.items : sms), kBwdThreads, smem, p2, st);
   if (e != ND_OK || a.splits == 1) return e;
   long long n4 = static_cast<long long>(batch) * sk * rk / 4;
   const float* part = a.part;
   void* p3[] = {&part, &dk, &dv, &n4, &a.splits};
   return attn_launch(bf ? (const void*)attn_dkv_join_kernel<__nv_bfloat16> : (const void*)attn_dkv_join_kernel<__half>,
-                     static_cast<int>((2 * n4 + 255) / 256), 256, 0, p3, st);
+                     dim3(static_cast<unsigned>((2 * n4 + 255) / 256)), 256, 0, p3, st);
 }
 
 }  // extern "C"

@@ -1,0 +1,293 @@
+// Attention of a few query rows per key head (a decoding step): the keys and values are read once, and that is all the
+// work there is - with one row a 128-row MMA tile is empty but for a line, and its softmax one busy warp.
+//
+// LPK lanes (the head's dimensions in 16-byte pieces, rounded up to a power of two) hold one key: its piece of K, then of
+// V, and the query rows' pieces in fp32. A score is 8 products per lane and a sum over the LPK lanes; every group of LPK
+// lanes ("slot") keeps its own running maximum, sum and output over the keys it sees, kUnroll of them at a time so that
+// 2 x kUnroll 16-byte loads are in flight per lane and the rescaling is paid once for all of them. Slots and warps are
+// joined at the end. Weights are never rounded; everything is 32-bit until the output.
+//
+// A CTA takes (sample, key head, range of keys): the sample's own keys cut evenly into as many ranges as it takes to give
+// every SM several CTAs. More than one range: normalised partial outputs and their log-sum-exp go through the workspace
+// to a second kernel. Bound: HBM (K and V once).
+#include "attn.cuh"
+
+namespace nd {
+
+constexpr int kFewThreads = 128;
+constexpr int kFewUnroll = 4;
+constexpr int kFewRows = 4;  // query rows per key head this kernel takes
+
+struct FewArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  float* lse;     // nullable, in the order of the tile kernels
+  float* part_o;  // [splits][batch][hkv][rows][d]
+  float* part_l;  // [splits][batch][hkv][rows]
+  AttnShape s;
+  AttnMask mask;
+  long long st[9];
+  float c;
+  int group, rows, splits;
+};
+
+// row r of key head h of sample b: its place in the padded order of the backward pass
+__device__ __forceinline__ long long lse_at(const FewArgs& a, int b, int h, int r) {
+  const int pos = r / a.group, head = h * a.group + r % a.group;
+  return (static_cast<long long>(b) * a.s.hb + head / a.s.gp) * a.s.rows_pad + pos * a.s.gp + head % a.s.gp;
+}
+
+// the rows that pad a head block to whole tiles count as empty
+__device__ __forceinline__ void pad_lse(const FewArgs& a, int b, int h) {
+  if (a.lse == nullptr) return;
+  const int blocks = a.group / a.s.gp, pad = a.s.rows_pad - a.s.rows;
+  for (int i = threadIdx.x; i < blocks * pad; i += blockDim.x)
+    a.lse[(static_cast<long long>(b) * a.s.hb + h * blocks + i / pad) * a.s.rows_pad + a.s.rows + i % pad] = -INFINITY;
+}
+
+template <typename T> __device__ __forceinline__ void unpack8(const uint4& w, float (&f)[8]) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float2 p = unpack_pair<T>(u[e]);
+    f[2 * e] = p.x;
+    f[2 * e + 1] = p.y;
+  }
+}
+
+template <typename T, int LPK, int R>
+__global__ void __launch_bounds__(kFewThreads) attn_few_kernel(const FewArgs a) {
+  constexpr int kSlots = 32 / LPK;                          // keys per warp and step
+  constexpr int kStep = kFewThreads / 32 * kSlots;          // keys per CTA and unrolled step
+  __shared__ float sh_o[kFewThreads / 32][R][LPK * 8];
+  __shared__ float sh_m[kFewThreads / 32][R], sh_l[kFewThreads / 32][R];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, piece = lane % LPK, slot = lane / LPK;
+  const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  griddep_launch_dependents();
+  griddep_wait();
+  const bool mine = piece * 8 < a.s.d;  // lanes behind the head's dimensions hold zeros
+  float q[R][8];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[r][e] = 0.f;
+    if (r < a.rows && mine) {
+      const int pos = r / a.group, head = h * a.group + r % a.group;
+      unpack8<T>(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.st[0] + pos * a.st[1] + head * a.st[2] + piece * 8)), q[r]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q[r][e] *= a.c;
+    }
+  }
+  const int n_keys = key_count(a.mask, b, a.s.sk, lane);
+  const int per = (n_keys + a.splits - 1) / a.splits;
+  const int first = split * per, end = first + per < n_keys ? first + per : n_keys;
+  const T* kp = static_cast<const T*>(a.k) + b * a.st[3] + h * a.st[5] + piece * 8;
+  const T* vp = static_cast<const T*>(a.v) + b * a.st[6] + h * a.st[8] + piece * 8;
+  const unsigned char* mask = a.mask.key_mask != nullptr ? a.mask.key_mask + static_cast<long long>(b) * a.s.sk : nullptr;
+  float m[R], l[R], o[R][8];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[r][e] = 0.f;
+  }
+  for (int k0 = first; k0 < end; k0 += kStep * kFewUnroll) {
+    uint4 kw[kFewUnroll], vw[kFewUnroll];
+    bool on[kFewUnroll];
+#pragma unroll
+    for (int u = 0; u < kFewUnroll; ++u) {
+      const int key = k0 + u * kStep + warp * kSlots + slot;
+      on[u] = key < end;
+      kw[u] = vw[u] = make_uint4(0, 0, 0, 0);
+      if (on[u] && mine) {
+        kw[u] = __ldcs(reinterpret_cast<const uint4*>(kp + static_cast<long long>(key) * a.st[4]));
+        vw[u] = __ldcs(reinterpret_cast<const uint4*>(vp + static_cast<long long>(key) * a.st[7]));
+      }
+      if (mask != nullptr && on[u]) on[u] = __ldg(mask + key) != 0;
+    }
+    float score[R][kFewUnroll];
+#pragma unroll
+    for (int u = 0; u < kFewUnroll; ++u) {
+      float kf[8];
+      unpack8<T>(kw[u], kf);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float x = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x = fmaf(q[r][e], kf[e], x);
+        score[r][u] = x;
+      }
+    }
+#pragma unroll
+    for (int d = LPK / 2; d >= 1; d >>= 1)
+#pragma unroll
+      for (int u = 0; u < kFewUnroll; ++u)
+#pragma unroll
+        for (int r = 0; r < R; ++r) score[r][u] += __shfl_xor_sync(0xffffffffu, score[r][u], d);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float top = m[r];
+#pragma unroll
+      for (int u = 0; u < kFewUnroll; ++u) {
+        score[r][u] = on[u] ? score[r][u] : -INFINITY;
+        top = max3(top, score[r][u], score[r][u]);
+      }
+      const float base = top == -INFINITY ? 0.f : top;
+      const float alpha = ex2_approx(m[r] - base);
+      m[r] = top;
+      l[r] *= alpha;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[r][e] *= alpha;
+#pragma unroll
+      for (int u = 0; u < kFewUnroll; ++u) {
+        score[r][u] = ex2_approx(score[r][u] - base);
+        l[r] += score[r][u];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kFewUnroll; ++u) {
+      float vf[8];
+      unpack8<T>(vw[u], vf);
+      if (!on[u]) {  // a key that takes no part may hold NaN
+#pragma unroll
+        for (int e = 0; e < 8; ++e) vf[e] = 0.f;
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[r][e] = fmaf(score[r][u], vf[e], o[r][e]);
+    }
+  }
+  // the slots of a warp, then the warps
+#pragma unroll
+  for (int d = LPK; d < 32; d <<= 1)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float mo = __shfl_xor_sync(0xffffffffu, m[r], d), lo = __shfl_xor_sync(0xffffffffu, l[r], d);
+      const float top = max3(m[r], mo, mo), base = top == -INFINITY ? 0.f : top;
+      const float wa = ex2_approx(m[r] - base), wb = ex2_approx(mo - base);
+      m[r] = top;
+      l[r] = l[r] * wa + lo * wb;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[r][e] = o[r][e] * wa + __shfl_xor_sync(0xffffffffu, o[r][e], d) * wb;
+    }
+  if (slot == 0) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sh_o[warp][r][piece * 8 + e] = o[r][e];
+      if (piece == 0) {
+        sh_m[warp][r] = m[r];
+        sh_l[warp][r] = l[r];
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.rows * a.s.d / 2; i += kFewThreads) {  // pairs of output elements
+    const int r = i / (a.s.d / 2), e = (i - r * (a.s.d / 2)) * 2;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kFewThreads / 32; ++w) top = max3(top, sh_m[w][r], sh_m[w][r]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+    for (int w = 0; w < kFewThreads / 32; ++w) {
+      const float wgt = ex2_approx(sh_m[w][r] - base);
+      sum = fmaf(sh_l[w][r], wgt, sum);
+      x = fmaf(sh_o[w][r][e], wgt, x);
+      y = fmaf(sh_o[w][r][e + 1], wgt, y);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (a.splits > 1) {
+      const long long at = ((static_cast<long long>(split) * a.s.batch + b) * a.s.hkv + h) * a.rows + r;
+      *reinterpret_cast<float2*>(a.part_o + at * a.s.d + e) = make_float2(x * inv, y * inv);
+      if (e == 0) a.part_l[at] = sum == 0.f ? -INFINITY : base + log2f(sum);
+    } else {
+      const int pos = r / a.group, head = h * a.group + r % a.group;
+      *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.s.sq + pos) * a.s.hq + head) * a.s.d + e) =
+          pack2<T>(x * inv, y * inv);
+      if (e == 0 && a.lse != nullptr) a.lse[lse_at(a, b, h, r)] = sum == 0.f ? -INFINITY : -(base + log2f(sum));
+    }
+  }
+  if (a.splits == 1) pad_lse(a, b, h);
+}
+
+// joins the ranges of one (sample, key head): a thread per pair of output elements
+template <typename T> __global__ void __launch_bounds__(kFewThreads) attn_few_join_kernel(const FewArgs a) {
+  const int h = blockIdx.x, b = blockIdx.y;
+  griddep_launch_dependents();
+  griddep_wait();
+  const long long n = static_cast<long long>(a.s.batch) * a.s.hkv * a.rows;
+  for (int i = threadIdx.x; i < a.rows * a.s.d / 2; i += kFewThreads) {
+    const int r = i / (a.s.d / 2), e = (i - r * (a.s.d / 2)) * 2;
+    const long long at = (static_cast<long long>(b) * a.s.hkv + h) * a.rows + r;
+    float top = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) top = max3(top, a.part_l[s * n + at], a.part_l[s * n + at]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, x = 0.f, y = 0.f;
+    for (int s = 0; s < a.splits; ++s) {  // a range without keys weighs 2^-inf and holds zeros
+      const float wgt = ex2_approx(a.part_l[s * n + at] - base);
+      const float2 o = *reinterpret_cast<const float2*>(a.part_o + (s * n + at) * a.s.d + e);
+      sum += wgt;
+      x = fmaf(o.x, wgt, x);
+      y = fmaf(o.y, wgt, y);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int pos = r / a.group, head = h * a.group + r % a.group;
+    *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + ((static_cast<long long>(b) * a.s.sq + pos) * a.s.hq + head) * a.s.d + e) =
+        pack2<T>(x * inv, y * inv);
+    if (e == 0 && a.lse != nullptr) a.lse[lse_at(a, b, h, r)] = sum == 0.f ? -INFINITY : -(base + log2f(sum));
+  }
+  pad_lse(a, b, h);
+}
+
+// ------------------------------------------------------------------ host side
+bool attn_few_takes(const AttnShape& s) { return s.sq <= kFewRows && s.sq * (s.hq / s.hkv) <= kFewRows; }
+
+static int few_splits(const AttnShape& s) {
+  // eight CTAs of 128 threads per SM keep enough loads in flight; a range of less than 64 keys is not worth a join
+  const long long pairs = static_cast<long long>(s.batch) * s.hkv, want = (8LL * sm_count() + pairs - 1) / pairs;
+  const long long most = s.sk / 64 > 1 ? s.sk / 64 : 1;
+  return static_cast<int>(want < most ? want : most);
+}
+
+size_t attn_few_ws(const AttnShape& s) {
+  const int splits = few_splits(s);
+  if (splits == 1) return 0;
+  return static_cast<size_t>(splits) * s.batch * s.hkv * s.sq * (s.hq / s.hkv) * (s.d + 1) * sizeof(float);
+}
+
+template <typename T, int R> static const void* pick_few(int d) {
+  if (d <= 8) return (const void*)attn_few_kernel<T, 1, R>;
+  if (d <= 16) return (const void*)attn_few_kernel<T, 2, R>;
+  if (d <= 32) return (const void*)attn_few_kernel<T, 4, R>;
+  if (d <= 64) return (const void*)attn_few_kernel<T, 8, R>;
+  return (const void*)attn_few_kernel<T, 16, R>;
+}
+template <typename T> static const void* pick_few_rows(int rows, int d) {
+  return rows == 1 ? pick_few<T, 1>(d) : rows == 2 ? pick_few<T, 2>(d) : pick_few<T, 4>(d);
+}
+
+int attn_few(int dtype, const void* q, const void* k, const void* v, void* out, float* lse, const AttnMask& mask,
+             const AttnShape& s, const int64_t* strides, float c, void* ws, cudaStream_t st) {
+  FewArgs a{};
+  a.q = q; a.k = k; a.v = v; a.out = out; a.lse = lse; a.s = s; a.mask = mask; a.c = c;
+  for (int i = 0; i < 9; ++i) a.st[i] = strides[i];
+  a.group = s.hq / s.hkv;
+  a.rows = s.sq * a.group;
+  a.splits = few_splits(s);
+  a.part_o = static_cast<float*>(ws);
+  a.part_l = a.part_o + static_cast<size_t>(a.splits) * s.batch * s.hkv * a.rows * s.d;
+  void* params[] = {&a};
+  const bool bf = dtype == ND_BF16;
+  const int e = attn_launch(bf ? pick_few_rows<__nv_bfloat16>(a.rows, s.d) : pick_few_rows<__half>(a.rows, s.d),
+                            dim3(a.splits, s.hkv, s.batch), kFewThreads, 0, params, st);
+  if (e != ND_OK || a.splits == 1) return e;
+  return attn_launch(bf ? (const void*)attn_few_join_kernel<__nv_bfloat16> : (const void*)attn_few_join_kernel<__half>,
+                     dim3(s.hkv, s.batch), kFewThreads, 0, params, st);
+}
+
+}  // namespace nd

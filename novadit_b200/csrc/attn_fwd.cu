@@ -496,7 +496,7 @@ template <typename T> static const void* pick_fwd(int kt) {
   }
 }
 
-int attn_launch(const void* fn, int grid, int threads, size_t smem, void** params, cudaStream_t st) {
+int attn_launch(const void* fn, dim3 grid, int threads, size_t smem, void** params, cudaStream_t st) {
   if (smem > 0) {
     const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) {
@@ -506,7 +506,7 @@ int attn_launch(const void* fn, int grid, int threads, size_t smem, void** param
     }
   }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -538,6 +538,7 @@ size_t nd_attn_fwd_ws_bytes(int64_t batch, int64_t sq, int64_t sk, int64_t hq, i
   if (nd::attn_check(ND_BF16, batch, sq, sk, hq, hkv, head_dim, 1.f) != ND_OK || batch == 0 || sq == 0) return 0;
   nd::FwdArgs a{};
   a.s = nd::attn_shape(batch, sq, sk, hq, hkv, head_dim);
+  if (nd::attn_few_takes(a.s)) return nd::attn_few_ws(a.s);
   nd::fwd_plan(a);
   return nd::fwd_ws(a);
 }
@@ -553,19 +554,26 @@ int nd_attn_fwd(int dtype, const void* q, const void* k, const void* v, void* ou
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   FwdArgs a{};
   a.s = attn_shape(batch, sq, sk, hq, hkv, head_dim);
-  fwd_plan(a);
   if (static_cast<long long>(a.s.sq) * a.s.gp > (1 << 30)) return ND_ERR_UNSUPPORTED;
-  const long long items = static_cast<long long>(a.s.batch) * a.s.hb * a.pairs * a.splits;
-  if (items > INT32_MAX / 2) return ND_ERR_UNSUPPORTED;
   if (!aligned16(q) || !aligned16(out) || (sk > 0 && (!aligned16(k) || !aligned16(v)))) return ND_ERR_UNSUPPORTED;
   for (int i = 0; i < 9; ++i)
     if (strides[i] < 0 || strides[i] % 8 != 0) return ND_ERR_UNSUPPORTED;
+  const AttnMask mask{static_cast<const unsigned char*>(key_mask), kv_lens};
+  const float c = scale * 1.4426950408889634f;
+  if (attn_few_takes(a.s)) {
+    const size_t need = attn_few_ws(a.s);
+    if (need > 0 && (ws == nullptr || ws_bytes < need || !aligned16(ws))) return ND_ERR_WORKSPACE;
+    return attn_few(dtype, q, k, v, out, lse, mask, a.s, strides, c, ws, st);
+  }
+  fwd_plan(a);
+  const long long items = static_cast<long long>(a.s.batch) * a.s.hb * a.pairs * a.splits;
+  if (items > INT32_MAX / 2) return ND_ERR_UNSUPPORTED;
   if (fwd_ws(a) > 0 && (ws == nullptr || ws_bytes < fwd_ws(a) || !aligned16(ws))) return ND_ERR_WORKSPACE;
   a.items = static_cast<int>(items);
-  a.mask = AttnMask{static_cast<const unsigned char*>(key_mask), kv_lens};
+  a.mask = mask;
   a.sink = WaitSink{nullptr, device_error_ptr()};
   a.lse = lse;
-  a.c = scale * 1.4426950408889634f;
+  a.c = c;
   a.part_o = static_cast<float*>(ws);
   a.part_l = a.splits > 1 ? a.part_o + static_cast<size_t>(a.splits) * a.s.batch * a.s.hb * a.s.rows_pad * a.s.d : nullptr;
   CUtensorMap mq, mk, mv, mo;
@@ -587,12 +595,12 @@ int nd_attn_fwd(int dtype, const void* q, const void* k, const void* v, void* ou
                                    : sizeof(FwdSmem<2, 80>)) + 1024;
   const int sms = sm_count();
   void* params[] = {&mq, &mk, &mv, &mo, &a};
-  int e = attn_launch(fn, a.items < sms ? a.items : sms, kFwdThreads, smem, params, st);
+  int e = attn_launch(fn, dim3(a.items < sms ? a.items : sms), kFwdThreads, smem, params, st);
   if (e != ND_OK || a.splits == 1) return e;
   const long long rows_all = static_cast<long long>(a.s.batch) * a.s.hb * a.s.rows_pad;
   void* jp[] = {&a, &out};
   return attn_launch(bf ? (const void*)attn_join_kernel<__nv_bfloat16> : (const void*)attn_join_kernel<__half>,
-                     static_cast<int>((rows_all + 7) / 8), 256, 0, jp, st);
+                     dim3(static_cast<unsigned>((rows_all + 7) / 8)), 256, 0, jp, st);
 }
 
 }  // extern "C"
