@@ -15,6 +15,9 @@
 namespace nd {
 
 constexpr int kFewThreads = 128;
+// CTAs per SM, by rows: what the registers of R query rows and their outputs leave (one row could have eight, which is more
+// rounds or more ranges of less: 34 us against 27 at 32 x 20 x 750 keys of 64)
+template <int R> constexpr int kFewCtas = R <= 2 ? 5 : 3;
 constexpr int kFewUnroll = 4;
 constexpr int kFewRows = 4;  // query rows per key head this kernel takes
 
@@ -47,52 +50,56 @@ __device__ __forceinline__ void pad_lse(const FewArgs& a, int b, int h) {
     a.lse[(static_cast<long long>(b) * a.s.hb + h * blocks + i / pad) * a.s.rows_pad + a.s.rows + i % pad] = -INFINITY;
 }
 
-template <typename T> __device__ __forceinline__ void unpack8(const uint4& w, float (&f)[8]) {
+template <typename T> __device__ __forceinline__ void unpack8(const uint4& w, uint64_t (&f)[4]) {
   const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const float2 p = unpack_pair<T>(u[e]);
-    f[2 * e] = p.x;
-    f[2 * e + 1] = p.y;
+    f[e] = f2_pack(p.x, p.y);
   }
 }
 
 template <typename T, int LPK, int R>
-__global__ void __launch_bounds__(kFewThreads) attn_few_kernel(const FewArgs a) {
+__global__ void __launch_bounds__(kFewThreads, kFewCtas<R>) attn_few_kernel(const FewArgs a) {
   constexpr int kSlots = 32 / LPK;                          // keys per warp and step
   constexpr int kStep = kFewThreads / 32 * kSlots;          // keys per CTA and unrolled step
-  __shared__ float sh_o[kFewThreads / 32][R][LPK * 8];
+  __shared__ alignas(8) float sh_o[kFewThreads / 32][R][LPK * 8];
   __shared__ float sh_m[kFewThreads / 32][R], sh_l[kFewThreads / 32][R];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, piece = lane % LPK, slot = lane / LPK;
   const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
   griddep_launch_dependents();
   griddep_wait();
   const bool mine = piece * 8 < a.s.d;  // lanes behind the head's dimensions hold zeros
-  float q[R][8];
+  uint4 qw[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) q[r][e] = 0.f;
+    qw[r] = make_uint4(0, 0, 0, 0);
     if (r < a.rows && mine) {
       const int pos = r / a.group, head = h * a.group + r % a.group;
-      unpack8<T>(__ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.st[0] + pos * a.st[1] + head * a.st[2] + piece * 8)), q[r]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) q[r][e] *= a.c;
+      qw[r] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + b * a.st[0] + pos * a.st[1] + head * a.st[2] + piece * 8));
     }
   }
   const int n_keys = key_count(a.mask, b, a.s.sk, lane);
+  uint64_t q[R][4];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    unpack8<T>(qw[r], q[r]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[r][e] = f2_mul(q[r][e], f2_pack(a.c, a.c));
+  }
   const int per = (n_keys + a.splits - 1) / a.splits;
   const int first = split * per, end = first + per < n_keys ? first + per : n_keys;
   const T* kp = static_cast<const T*>(a.k) + b * a.st[3] + h * a.st[5] + piece * 8;
   const T* vp = static_cast<const T*>(a.v) + b * a.st[6] + h * a.st[8] + piece * 8;
   const unsigned char* mask = a.mask.key_mask != nullptr ? a.mask.key_mask + static_cast<long long>(b) * a.s.sk : nullptr;
-  float m[R], l[R], o[R][8];
+  float m[R], l[R];
+  uint64_t o[R][4];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     m[r] = -INFINITY;
     l[r] = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[r][e] = 0.f;
+    for (int e = 0; e < 4; ++e) o[r][e] = 0;
   }
   for (int k0 = first; k0 < end; k0 += kStep * kFewUnroll) {
     uint4 kw[kFewUnroll], vw[kFewUnroll];
@@ -111,14 +118,15 @@ __global__ void __launch_bounds__(kFewThreads) attn_few_kernel(const FewArgs a) 
     float score[R][kFewUnroll];
 #pragma unroll
     for (int u = 0; u < kFewUnroll; ++u) {
-      float kf[8];
+      uint64_t kf[4];
       unpack8<T>(kw[u], kf);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        float x = 0.f;
+        uint64_t x = f2_mul(q[r][0], kf[0]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x = fmaf(q[r][e], kf[e], x);
-        score[r][u] = x;
+        for (int e = 1; e < 4; ++e) x = f2_fma(q[r][e], kf[e], x);
+        const float2 y = f2_unpack(x);
+        score[r][u] = y.x + y.y;
       }
     }
 #pragma unroll
@@ -140,7 +148,7 @@ __global__ void __launch_bounds__(kFewThreads) attn_few_kernel(const FewArgs a) 
       m[r] = top;
       l[r] *= alpha;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[r][e] *= alpha;
+      for (int e = 0; e < 4; ++e) o[r][e] = f2_mul(o[r][e], f2_pack(alpha, alpha));
 #pragma unroll
       for (int u = 0; u < kFewUnroll; ++u) {
         score[r][u] = ex2_approx(score[r][u] - base);
@@ -149,16 +157,12 @@ __global__ void __launch_bounds__(kFewThreads) attn_few_kernel(const FewArgs a) 
     }
 #pragma unroll
     for (int u = 0; u < kFewUnroll; ++u) {
-      float vf[8];
-      unpack8<T>(vw[u], vf);
-      if (!on[u]) {  // a key that takes no part may hold NaN
-#pragma unroll
-        for (int e = 0; e < 8; ++e) vf[e] = 0.f;
-      }
+      uint64_t vf[4];
+      unpack8<T>(on[u] ? vw[u] : make_uint4(0, 0, 0, 0), vf);  // a key that takes no part may hold NaN
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[r][e] = fmaf(score[r][u], vf[e], o[r][e]);
+        for (int e = 0; e < 4; ++e) o[r][e] = f2_fma(f2_pack(score[r][u], score[r][u]), vf[e], o[r][e]);
     }
   }
   // the slots of a warp, then the warps
@@ -172,13 +176,14 @@ __global__ void __launch_bounds__(kFewThreads) attn_few_kernel(const FewArgs a) 
       m[r] = top;
       l[r] = l[r] * wa + lo * wb;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[r][e] = o[r][e] * wa + __shfl_xor_sync(0xffffffffu, o[r][e], d) * wb;
+      for (int e = 0; e < 4; ++e)
+        o[r][e] = f2_fma(__shfl_xor_sync(0xffffffffu, o[r][e], d), f2_pack(wb, wb), f2_mul(o[r][e], f2_pack(wa, wa)));
     }
   if (slot == 0) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sh_o[warp][r][piece * 8 + e] = o[r][e];
+      for (int e = 0; e < 4; ++e) *reinterpret_cast<float2*>(&sh_o[warp][r][piece * 8 + 2 * e]) = f2_unpack(o[r][e]);
       if (piece == 0) {
         sh_m[warp][r] = m[r];
         sh_l[warp][r] = l[r];
@@ -245,17 +250,45 @@ template <typename T> __global__ void __launch_bounds__(kFewThreads) attn_few_jo
 }
 
 // ------------------------------------------------------------------ host side
-bool attn_few_takes(const AttnShape& s) { return s.sq <= kFewRows && s.sq * (s.hq / s.hkv) <= kFewRows; }
+// Up to two rows always (one row: 76 us against 91 us of the tile kernel at 2 x 8 heads x 50021 keys of 128, 34 against 59
+// at 32 x 20 x 750 x 64; two rows: 76 / 90 and 27 / 59). With three or four the arithmetic counts: short keys only (32 x 16
+// x 77 x 72, four rows: 12.7 us against 19.1, 64 x 4 x 300 x 64: 11.9 / 18.7; but 64 x 16 x 300 x 128, three rows: 68 / 56,
+// 2 x 8 x 50021 x 128, four rows: 139 / 90).
+bool attn_few_takes(const AttnShape& s) {
+  const int group = s.hq / s.hkv;
+  if (s.sq > kFewRows || group > kFewRows || s.sq * group > kFewRows) return false;
+  return s.sq * group <= 2 || static_cast<long long>(s.sk) * s.d <= 32768;
+}
 
-static int few_splits(const AttnShape& s) {
-  // eight CTAs of 128 threads per SM keep enough loads in flight; a range of less than 64 keys is not worth a join
-  const long long pairs = static_cast<long long>(s.batch) * s.hkv, want = (8LL * sm_count() + pairs - 1) / pairs;
+static int few_splits(const AttnShape& s, bool varies) {
+  // CTAs run in rounds of what the GPU holds at once. Less than half a round: as many ranges as fill one (2 x 8 key heads x
+  // 50021 keys: 98 us with 1.1 rounds, 76 us with one), none below 64 keys. More: the fewest ranges of 512 keys and more that
+  // fill four fifths of their rounds, else the best filled; shorter ranges do not pay for the second kernel (64 x 4 x 300
+  // keys: 16 us in three ranges, 12 in one). Where lengths differ the longest sample's CTA would be the last one running:
+  // one and a half rounds' worth of ranges, none below 256 keys (32 x 20 x up to 1500 keys: 42 us in one range, 31 in two).
+  const int rows = s.sq * (s.hq / s.hkv), ctas = rows == 1 ? kFewCtas<1> : rows == 2 ? kFewCtas<2> : kFewCtas<4>;
+  const long long pairs = static_cast<long long>(s.batch) * s.hkv, room = static_cast<long long>(ctas) * sm_count();
   const long long most = s.sk / 64 > 1 ? s.sk / 64 : 1;
-  return static_cast<int>(want < most ? want : most);
+  if (pairs * 2 <= room) return static_cast<int>(room / pairs < most ? room / pairs : most);
+  if (varies) {
+    const long long n = (room * 3 / 2 + pairs - 1) / pairs, top = s.sk / 256 > 1 ? s.sk / 256 : 1;
+    return static_cast<int>(n < top ? n : top);
+  }
+  int best = 1;
+  double best_fill = 0;
+  for (int n = 1; n <= 8 && (n == 1 || s.sk / n >= 512); ++n) {
+    const double fill = static_cast<double>(pairs * n) / static_cast<double>((pairs * n + room - 1) / room * room);
+    if (fill > best_fill - 1e-9) {
+      best = n;
+      best_fill = fill;
+    }
+    if (fill >= 0.8) break;
+  }
+  return best;
 }
 
 size_t attn_few_ws(const AttnShape& s) {
-  const int splits = few_splits(s);
+  const int one = few_splits(s, false), other = few_splits(s, true), splits = one > other ? one : other;
   if (splits == 1) return 0;
   return static_cast<size_t>(splits) * s.batch * s.hkv * s.sq * (s.hq / s.hkv) * (s.d + 1) * sizeof(float);
 }
@@ -278,7 +311,7 @@ int attn_few(int dtype, const void* q, const void* k, const void* v, void* out, 
   for (int i = 0; i < 9; ++i) a.st[i] = strides[i];
   a.group = s.hq / s.hkv;
   a.rows = s.sq * a.group;
-  a.splits = few_splits(s);
+  a.splits = few_splits(s, mask.key_mask != nullptr || mask.kv_lens != nullptr);
   a.part_o = static_cast<float*>(ws);
   a.part_l = a.part_o + static_cast<size_t>(a.splits) * s.batch * s.hkv * a.rows * s.d;
   void* params[] = {&a};
