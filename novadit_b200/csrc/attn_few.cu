@@ -15,9 +15,8 @@
 namespace nd {
 
 constexpr int kFewThreads = 128;
-// CTAs per SM, by rows: what the registers of R query rows and their outputs leave (one row could have eight, which is more
-// rounds or more ranges of less: 34 us against 27 at 32 x 20 x 750 keys of 64)
-template <int R> constexpr int kFewCtas = R <= 2 ? 5 : 3;
+// CTAs per SM, by rows: what the registers of R query rows, their outputs and the loads in flight leave without spills
+template <int R> constexpr int kFewCtas = R == 1 ? 6 : R == 2 ? 5 : 3;
 constexpr int kFewUnroll = 4;
 constexpr int kFewRows = 4;  // query rows per key head this kernel takes
 
@@ -265,13 +264,13 @@ static int few_splits(const AttnShape& s, bool varies) {
   // 50021 keys: 98 us with 1.1 rounds, 76 us with one), none below 64 keys. More: the fewest ranges of 512 keys and more that
   // fill four fifths of their rounds, else the best filled; shorter ranges do not pay for the second kernel (64 x 4 x 300
   // keys: 16 us in three ranges, 12 in one). Where lengths differ the longest sample's CTA would be the last one running:
-  // one and a half rounds' worth of ranges, none below 256 keys (32 x 20 x up to 1500 keys: 42 us in one range, 31 in two).
+  // a round and a quarter of ranges, none below 256 keys (32 x 20 x up to 1500 keys: 42 us in one range, 31 in two).
   const int rows = s.sq * (s.hq / s.hkv), ctas = rows == 1 ? kFewCtas<1> : rows == 2 ? kFewCtas<2> : kFewCtas<4>;
   const long long pairs = static_cast<long long>(s.batch) * s.hkv, room = static_cast<long long>(ctas) * sm_count();
   const long long most = s.sk / 64 > 1 ? s.sk / 64 : 1;
   if (pairs * 2 <= room) return static_cast<int>(room / pairs < most ? room / pairs : most);
   if (varies) {
-    const long long n = (room * 3 / 2 + pairs - 1) / pairs, top = s.sk / 256 > 1 ? s.sk / 256 : 1;
+    const long long n = (room * 5 / 4 + pairs - 1) / pairs, top = s.sk / 256 > 1 ? s.sk / 256 : 1;
     return static_cast<int>(n < top ? n : top);
   }
   int best = 1;
