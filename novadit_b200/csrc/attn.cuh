@@ -135,13 +135,31 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
-// D = A B^T over `steps` K = 16 steps of two K-major tiles, B of ROWS rows
-template <int ROWS = kTile>
-__device__ __forceinline__ void issue_nt(uint32_t d, uint64_t a, uint64_t b, int steps, uint32_t idesc) {
+// A run of MMAs from shared memory without a branch between them. With one (a test of the step count before each) an MMA
+// takes 75 cycles at N = 64 and 107 at N = 128 instead of 48 and 64: the issue of the next then waits for the one before. So
+// the step count is a constant of the whole issue loop for the usual head sizes (forward + backward at 2 x 16 x 4096^2 x 64:
+// 884 us against 822; as a switch in front of every run it costs more than it gives, 1003 us).
+template <int STEPS, int ROWS> __device__ __forceinline__ void run_nt(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
   mma_ss(d, a, b, idesc, 0u);
 #pragma unroll
-  for (int k = 1; k < 8; ++k)
-    if (k < steps) mma_ss(d, a + step_k(k), b + step_k<ROWS>(k), idesc, 1u);
+  for (int k = 1; k < STEPS; ++k) mma_ss(d, a + step_k(k), b + step_k<ROWS>(k), idesc, 1u);
+}
+// D = A B^T over STEPS K = 16 steps of two K-major tiles, B of ROWS rows; STEPS 0: `steps` of them
+template <int STEPS, int ROWS = kTile>
+__device__ __forceinline__ void issue_nt(uint32_t d, uint64_t a, uint64_t b, int steps, uint32_t idesc) {
+  if constexpr (STEPS > 0) {
+    run_nt<STEPS, ROWS>(d, a, b, idesc);
+  } else {
+    mma_ss(d, a, b, idesc, 0u);
+    for (int k = 1; k < steps; ++k) mma_ss(d, a + step_k(k), b + step_k<ROWS>(k), idesc, 1u);
+  }
+}
+// calls f with the step count as a constant where it is one of the usual ones (heads of 64, 72 / 80 and 128)
+template <typename F> __device__ __forceinline__ void with_steps(int steps, F&& f) {
+  if (steps == 4) f(std::integral_constant<int, 4>{});
+  else if (steps == 5) f(std::integral_constant<int, 5>{});
+  else if (steps == 8) f(std::integral_constant<int, 8>{});
+  else f(std::integral_constant<int, 0>{});
 }
 // D (+)= A B over `steps` groups of 16 rows of B: A from tensor memory, 8 columns per step, every GROUP steps `stride` columns
 // behind the ones before

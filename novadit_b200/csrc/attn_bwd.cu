@@ -204,6 +204,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     const uint64_t res = desc_k(smem_u32(s.res[0])), ring = desc_k(smem_u32(s.ring[0])), ring_mn = desc_mn<>(smem_u32(s.ring[0]));
     constexpr uint32_t kStep = kTileBytes >> 4;
     constexpr uint32_t kHalfRows = 64 * 128 >> 4;  // the second half of a tile's rows
+    with_steps(ksteps, [&](auto ks) {
     int it = 0, cnt = 0, o_cnt = 0;
     uint32_t done[2] = {0, 0};  // key tiles of the items before, per half
     bool ok = true;
@@ -226,14 +227,14 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           const int k_at = it1 + 2 * j;
           if (!full(k_at, 125)) return;
           tc_fence_after();
-          issue_nt(tmem + h * 64, res, ring + (k_at % kRing) * kStep + h * kHalfRows, ksteps, attn_idesc(kFmt, keys(j, h), false));
+          issue_nt<decltype(ks)::value>(tmem + h * 64, res, ring + (k_at % kRing) * kStep + h * kHalfRows, ksteps, attn_idesc(kFmt, keys(j, h), false));
           mma_commit(&s.s_full[h]);
         };
         auto issue_dp = [&](int j, int h) {
           const int v_at = it1 + 2 * j + 1;
           if (!full(v_at, 127)) return;
           tc_fence_after();
-          issue_nt(tmem + 128 + h * 64, res + kStep, ring + (v_at % kRing) * kStep + h * kHalfRows, ksteps,
+          issue_nt<decltype(ks)::value>(tmem + 128 + h * 64, res + kStep, ring + (v_at % kRing) * kStep + h * kHalfRows, ksteps,
                    attn_idesc(kFmt, keys(j, h), false));
           mma_commit(&s.dp_full[h]);
         };
@@ -300,6 +301,7 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
       o_cnt += (w.o || kHalf) ? 1 : 0;
       ++cnt;
     }
+    });
     __syncwarp();
    }
   } else {
@@ -551,6 +553,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const uint64_t res = desc_k(smem_u32(s.res[0])), ring = desc_k(smem_u32(s.ring[0])), ring_mn = desc_mn<>(smem_u32(s.ring[0]));
     constexpr uint32_t kStep = kTileBytes >> 4;
     constexpr uint32_t kHalfRows = 64 * 128 >> 4;  // the second half of a tile's rows
+    with_steps(ksteps, [&](auto ks) {
     int it = 0, cnt = 0;
     uint32_t done = 0;  // query tiles of the items before
     bool ok = true;
@@ -567,14 +570,14 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
           const int q_at = it + 2 * i;
           if (!full(q_at, 146)) return;
           tc_fence_after();
-          issue_nt(tmem + h * 64, res, ring + (q_at % kRing) * kStep + h * kHalfRows, ksteps, id_s);
+          issue_nt<decltype(ks)::value>(tmem + h * 64, res, ring + (q_at % kRing) * kStep + h * kHalfRows, ksteps, id_s);
           mma_commit(&s.s_full[h]);
         };
         auto issue_dp = [&](int i, int h) {
           const int d_at = it + 2 * i + 1;
           if (!full(d_at, 148)) return;
           tc_fence_after();
-          issue_nt(tmem + 128 + h * 64, res + kStep, ring + (d_at % kRing) * kStep + h * kHalfRows, ksteps, id_s);
+          issue_nt<decltype(ks)::value>(tmem + 128 + h * 64, res + kStep, ring + (d_at % kRing) * kStep + h * kHalfRows, ksteps, id_s);
           mma_commit(&s.dp_full[h]);
           if (h == 1 && i + 1 == w.n_i) mma_commit(&s.res_empty);
         };
@@ -619,6 +622,7 @@ attn_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       done += w.n_i;
       ++cnt;
     }
+    });
     __syncwarp();
    }
   } else {

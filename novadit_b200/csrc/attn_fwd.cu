@@ -160,6 +160,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const int ksteps = a.s.dn / 16;
     const uint32_t id_o = attn_idesc(kFmt, a.s.dn, true);
     const uint64_t q_desc = desc_k(smem_u32(s.q[0])), k_desc = desc_k(smem_u32(s.kv[0])), v_desc = desc_mn<KT>(smem_u32(s.kv[0]));
+    with_steps(ksteps, [&](auto ks) {
     int it = 0, q_cnt = 0;
     uint32_t base[2] = {0, 0};  // key tiles of the items before, per query tile
     bool ok = true;
@@ -187,7 +188,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
               if (ok && n > 0) ok = mbar_wait(&s.s_free[t], (n - 1) & 1, abort_flag, a.sink, 104);
               if (!ok) break;
               tc_fence_after();
-              issue_nt<KT>(tmem + t * KT, q_desc + t * (kQBytes >> 4), k_desc + (k_at % kKv) * (kKvBytes >> 4), ksteps, id_s);
+              issue_nt<decltype(ks)::value, KT>(tmem + t * KT, q_desc + t * (kQBytes >> 4), k_desc + (k_at % kKv) * (kKvBytes >> 4), ksteps, id_s);
               mma_commit(&s.s_full[t]);
               if (t == nt - 1) {
                 mma_commit(&s.kv_empty[k_at % kKv]);
@@ -213,6 +214,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
       if (w.two) base[1] += w.n_t;
       ++q_cnt;
     }
+    });
     __syncwarp();
    }
   } else {
