@@ -7,11 +7,12 @@
 // becomes a 64-bit fixed-point fraction of a turn, and position * fraction is ONE 64-bit integer product whose overflow
 // drops the whole turns: the remainder is exact, whatever the position. Its top 32 bits go to sincospi.
 //
-// Bound: HBM, one read and one write of every element (plus one position per token and axis). A CTA takes TT tokens:
-// it fills a table of TT x R (cos, sin) in shared memory once, and all heads (of q and k) read it, so a sine costs the
-// kernel 1 / heads of what it would cost per element. A thread then owns one vector slot of the token (a pair of
-// vectors R apart in the half layout, one vector of adjacent pairs in the interleaved one, a plain copy elsewhere) and
-// walks the TT tokens with it: the slot's address is decoded once, and the loads of the TT tokens are in flight together.
+// Bound: HBM, one read and one write of every element (plus one position per token and axis). A CTA takes kRotTokens
+// tokens and fills a table of kRotTokens x R (cos, sin) in shared memory once; all heads of q and k read it, so a sine costs
+// the kernel 1 / heads of what it would cost per element. A thread owns one vector slot of the token (a pair of vectors R
+// apart in the half layout, one vector of adjacent pairs in the interleaved one, a plain copy elsewhere), of q and of k
+// alike, and one 16-byte slot of v. The loads of its first slots, of all the CTA's tokens, are issued before the table is
+// worked out and are in flight meanwhile: with the table first a CTA waits for memory four times in a row.
 #include "common.cuh"
 
 namespace nd {
@@ -25,17 +26,16 @@ struct RotSeg {  // one tensor of [tokens, heads, D]; strides in elements
   void* dst;
   long long src_b, src_s, src_h;
   long long dst_b, dst_s, dst_h;
-  int rotate;
 };
 
 struct RotArgs {
-  RotSeg seg[3];
+  RotSeg seg[3];          // the rotated ones (one or two), then the copied one
   const void* positions;  // [B or 1, S, axes] of pos_bytes-byte integers, contiguous within a sample
   const double* freqs;    // [axes, pairs / axes] radians per position
   long long tokens, seq_len, pos_b;  // pos_b: elements between samples (0: shared)
-  int n_seg, heads, head_dim, pairs, axes, pos_bytes;
+  int heads, head_dim, pairs, axes, pos_bytes;
   int rot_units, units;   // vector slots per head of a rotated segment: rotated ones, all
-  int copy_units;         // vector slots per head of a copied segment
+  int copy_units;         // 16-byte (or narrower) slots per head of the copied segment
   unsigned units_mul, copy_mul;  // slot / units as a high product (0: units == 1)
   float factor;
   int inverse;
@@ -67,24 +67,110 @@ __device__ __forceinline__ int rot_div(int n, unsigned mul) {
   return mul == 0 ? n : static_cast<int>(__umulhi(static_cast<unsigned>(n), mul));
 }
 
-template <typename T, int V, bool ALIGNED, bool INTERLEAVED>
+// ROT rotated segments (x, or q and k), COPY: a copied one behind them (v), in vectors of CV elements
+template <typename T, int V, int CV, bool ALIGNED, bool INTERLEAVED, int ROT, bool COPY>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotArgs a) {
   extern __shared__ float2 table[];  // [kRotTokens][pairs]
-  __shared__ long long src_off[3][kRotTokens], dst_off[3][kRotTokens];
+  constexpr int kParts = INTERLEAVED ? 1 : 2;  // vectors per rotated slot
   const long long t0 = static_cast<long long>(blockIdx.x) * kRotTokens;
   const int nt = a.tokens - t0 < kRotTokens ? static_cast<int>(a.tokens - t0) : kRotTokens;
-  for (int i = threadIdx.x; i < a.n_seg * kRotTokens; i += blockDim.x) {
-    const int g = i / kRotTokens, j = i - g * kRotTokens;
-    if (j < nt) {
-      const long long b = (t0 + j) / a.seq_len, s = (t0 + j) - b * a.seq_len;
-      src_off[g][j] = b * a.seg[g].src_b + s * a.seg[g].src_s;
-      dst_off[g][j] = b * a.seg[g].dst_b + s * a.seg[g].dst_s;
+  // sample and position of the CTA's tokens: one division (a 64-bit one is a hundred instructions), then steps
+  const long long b0 = a.tokens <= 0x7FFFFFFFLL ? static_cast<long long>(static_cast<unsigned>(t0) / static_cast<unsigned>(a.seq_len))
+                                                : t0 / a.seq_len;
+  const long long s0 = t0 - b0 * a.seq_len;
+  auto place = [&](int j, long long& b, long long& s) {
+    b = b0;
+    s = s0 + j;
+    while (s >= a.seq_len) {
+      s -= a.seq_len;
+      ++b;
     }
+  };
+  long long tok_b[kRotTokens], tok_s[kRotTokens];
+#pragma unroll
+  for (int j = 0; j < kRotTokens; ++j) place(j, tok_b[j], tok_s[j]);
+  Vec<T, V> x[ROT][kRotTokens][kParts];
+  auto load = [&](int i) {
+    const int head = rot_div(i, a.units_mul), u = i - head * a.units;
+    const bool rotated = u < a.rot_units;
+    const int e0 = rotated ? u * V : 2 * a.pairs + (u - a.rot_units) * V;
+#pragma unroll
+    for (int g = 0; g < ROT; ++g) {
+      const T* src = static_cast<const T*>(a.seg[g].src) + head * a.seg[g].src_h + e0;
+#pragma unroll
+      for (int j = 0; j < kRotTokens; ++j)
+        if (j < nt) {
+          const T* at = src + tok_b[j] * a.seg[g].src_b + tok_s[j] * a.seg[g].src_s;
+          rot_load<T, V, ALIGNED>(x[g][j][0], at);
+          if (kParts == 2 && rotated) rot_load<T, V, ALIGNED>(x[g][j][kParts - 1], at + a.pairs);
+        }
+    }
+  };
+  auto finish = [&](int i) {
+    const int head = rot_div(i, a.units_mul), u = i - head * a.units;
+    const bool rotated = u < a.rot_units;
+    const int e0 = rotated ? u * V : 2 * a.pairs + (u - a.rot_units) * V;
+#pragma unroll
+    for (int g = 0; g < ROT; ++g) {
+      T* dst = static_cast<T*>(a.seg[g].dst) + head * a.seg[g].dst_h + e0;
+#pragma unroll
+      for (int j = 0; j < kRotTokens; ++j) {
+        if (j >= nt) break;
+        T* at = dst + tok_b[j] * a.seg[g].dst_b + tok_s[j] * a.seg[g].dst_s;
+        if (rotated) {
+          const float2* tab = table + j * a.pairs;
+          float f[kParts][V];
+          x[g][j][0].unpack(f[0]);
+          if constexpr (INTERLEAVED) {
+#pragma unroll
+            for (int e = 0; e < V; e += 2) {
+              const float2 cs = tab[(u * V + e) / 2];
+              const float re = f[0][e], im = f[0][e + 1];
+              f[0][e] = rot_re(re, im, cs);
+              f[0][e + 1] = rot_im(re, im, cs);
+            }
+          } else {
+            x[g][j][kParts - 1].unpack(f[kParts - 1]);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              const float2 cs = tab[u * V + e];
+              const float re = f[0][e], im = f[kParts - 1][e];
+              f[0][e] = rot_re(re, im, cs);
+              f[kParts - 1][e] = rot_im(re, im, cs);
+            }
+            x[g][j][kParts - 1].pack(f[kParts - 1]);
+            rot_store<T, V, ALIGNED>(x[g][j][kParts - 1], at + a.pairs);
+          }
+          x[g][j][0].pack(f[0]);
+        }
+        rot_store<T, V, ALIGNED>(x[g][j][0], at);
+      }
+    }
+  };
+  Vec<T, CV> y[COPY ? kRotTokens : 1];
+  auto copy = [&](int i, bool store) {
+    const int head = rot_div(i, a.copy_mul), e0 = (i - head * a.copy_units) * CV;
+    const RotSeg& sg = a.seg[ROT];
+#pragma unroll
+    for (int j = 0; j < kRotTokens; ++j) {
+      if (j >= nt) break;
+      if (!store) rot_load<T, CV, ALIGNED>(y[COPY ? j : 0], static_cast<const T*>(sg.src) + tok_b[j] * sg.src_b + tok_s[j] * sg.src_s + head * sg.src_h + e0);
+      else rot_store<T, CV, ALIGNED>(y[COPY ? j : 0], static_cast<T*>(sg.dst) + tok_b[j] * sg.dst_b + tok_s[j] * sg.dst_s + head * sg.dst_h + e0);
+    }
+  };
+
+  const int n_rot = a.heads * a.units, n_copy = COPY ? a.heads * a.copy_units : 0;
+  int i = threadIdx.x, c = threadIdx.x;
+  if (i < n_rot) load(i);
+  if constexpr (COPY) {
+    if (c < n_copy) copy(c, false);
   }
+
   const int per_axis = a.pairs / a.axes;
-  for (int i = threadIdx.x; i < nt * a.pairs; i += blockDim.x) {
-    const int j = i / a.pairs, p = i - j * a.pairs;
-    const long long b = (t0 + j) / a.seq_len, s = (t0 + j) - b * a.seq_len;
+  for (int k = threadIdx.x; k < nt * a.pairs; k += blockDim.x) {
+    const int j = k / a.pairs, p = k - j * a.pairs;
+    long long b, s;
+    place(j, b, s);
     const long long at = b * a.pos_b + s * a.axes + p / per_axis;
     const long long pos = a.pos_bytes == 8 ? __ldg(static_cast<const long long*>(a.positions) + at)
                                            : static_cast<long long>(__ldg(static_cast<const int*>(a.positions) + at));
@@ -94,103 +180,47 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotArgs a) {
     float sn, cs;
     sincospif(static_cast<float>(static_cast<int>(turn >> 32)) * 4.656612873077392578125e-10f, &sn, &cs);  // 2^-31
     if (!isfinite(f)) sn = cs = __int_as_float(0x7fffffff);
-    table[i] = make_float2(cs * a.factor, (a.inverse ? -sn : sn) * a.factor);
+    table[k] = make_float2(cs * a.factor, (a.inverse ? -sn : sn) * a.factor);
   }
   __syncthreads();
 
-  for (int g = 0; g < a.n_seg; ++g) {
-    const RotSeg& sg = a.seg[g];
-    const int rot_units = sg.rotate ? a.rot_units : 0, units = sg.rotate ? a.units : a.copy_units;
-    const unsigned mul = sg.rotate ? a.units_mul : a.copy_mul;
-    const T* src = static_cast<const T*>(sg.src);
-    T* dst = static_cast<T*>(sg.dst);
-    for (int i = threadIdx.x; i < a.heads * units; i += blockDim.x) {
-      const int head = rot_div(i, mul), u = i - head * units;
-      const long long hs = head * sg.src_h, hd = head * sg.dst_h;
-      if (u < rot_units) {
-        if constexpr (INTERLEAVED) {
-          Vec<T, V> x[kRotTokens];
-#pragma unroll
-          for (int j = 0; j < kRotTokens; ++j)
-            if (j < nt) rot_load<T, V, ALIGNED>(x[j], src + src_off[g][j] + hs + u * V);
-#pragma unroll
-          for (int j = 0; j < kRotTokens; ++j) {
-            if (j >= nt) break;
-            float f[V];
-            x[j].unpack(f);
-#pragma unroll
-            for (int e = 0; e < V; e += 2) {
-              const float2 cs = table[j * a.pairs + (u * V + e) / 2];
-              const float re = f[e], im = f[e + 1];
-              f[e] = rot_re(re, im, cs);
-              f[e + 1] = rot_im(re, im, cs);
-            }
-            x[j].pack(f);
-            rot_store<T, V, ALIGNED>(x[j], dst + dst_off[g][j] + hd + u * V);
-          }
-        } else {
-          Vec<T, V> x[kRotTokens], y[kRotTokens];
-#pragma unroll
-          for (int j = 0; j < kRotTokens; ++j)
-            if (j < nt) {
-              rot_load<T, V, ALIGNED>(x[j], src + src_off[g][j] + hs + u * V);
-              rot_load<T, V, ALIGNED>(y[j], src + src_off[g][j] + hs + a.pairs + u * V);
-            }
-#pragma unroll
-          for (int j = 0; j < kRotTokens; ++j) {
-            if (j >= nt) break;
-            float fx[V], fy[V];
-            x[j].unpack(fx);
-            y[j].unpack(fy);
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-              const float2 cs = table[j * a.pairs + u * V + e];
-              const float re = fx[e], im = fy[e];
-              fx[e] = rot_re(re, im, cs);
-              fy[e] = rot_im(re, im, cs);
-            }
-            x[j].pack(fx);
-            y[j].pack(fy);
-            rot_store<T, V, ALIGNED>(x[j], dst + dst_off[g][j] + hd + u * V);
-            rot_store<T, V, ALIGNED>(y[j], dst + dst_off[g][j] + hd + a.pairs + u * V);
-          }
-        }
-      } else {  // a slot that is copied: the rest of a rotated head, or a head of v
-        const int e0 = sg.rotate ? 2 * a.pairs + (u - rot_units) * V : u * V;
-        Vec<T, V> x[kRotTokens];
-#pragma unroll
-        for (int j = 0; j < kRotTokens; ++j)
-          if (j < nt) rot_load<T, V, ALIGNED>(x[j], src + src_off[g][j] + hs + e0);
-#pragma unroll
-        for (int j = 0; j < kRotTokens; ++j)
-          if (j < nt) rot_store<T, V, ALIGNED>(x[j], dst + dst_off[g][j] + hd + e0);
-      }
+  while (i < n_rot) {
+    finish(i);
+    i += blockDim.x;
+    if (i < n_rot) load(i);
+  }
+  if constexpr (COPY) {
+    while (c < n_copy) {
+      copy(c, true);
+      c += blockDim.x;
+      if (c < n_copy) copy(c, false);
     }
   }
 }
 
 static unsigned rot_mul(int d) { return d <= 1 ? 0u : static_cast<unsigned>((0x100000000ull + d - 1) / d); }
 
-template <typename T, int V, bool ALIGNED>
-static int rot_launch_v(RotArgs& a, bool interleaved, cudaStream_t st) {
+template <typename T, int V, int CV, bool ALIGNED>
+static int rot_launch_v(RotArgs& a, bool interleaved, bool pack, cudaStream_t st) {
   const int rest = a.head_dim - 2 * a.pairs;
   a.rot_units = interleaved ? 2 * a.pairs / V : a.pairs / V;
   a.units = a.rot_units + rest / V;
-  a.copy_units = a.head_dim / V;
+  a.copy_units = a.head_dim / CV;
   a.units_mul = rot_mul(a.units);
   a.copy_mul = rot_mul(a.copy_units);
   const long long all = static_cast<long long>(a.heads) * (a.units > a.copy_units ? a.units : a.copy_units);
   if (all >= 65536) return ND_ERR_UNSUPPORTED;  // rot_div's range
-  const int slots = static_cast<int>(all);
   const long long grid = (a.tokens + kRotTokens - 1) / kRotTokens;
   if (grid > 0x7FFFFFFFLL) return ND_ERR_UNSUPPORTED;
+  const int slots = a.heads * a.units;
   const int passes = (slots + kRotThreads - 1) / kRotThreads;
-  int nt = ((slots + passes - 1) / passes + 31) / 32 * 32;
+  const int nt = ((slots + passes - 1) / passes + 31) / 32 * 32;
   const void* fn;
   if constexpr (V == 1) {  // an interleaved pair needs two elements
-    fn = (const void*)rotary_kernel<T, V, ALIGNED, false>;
+    fn = pack ? (const void*)rotary_kernel<T, V, CV, ALIGNED, false, 2, true> : (const void*)rotary_kernel<T, V, CV, ALIGNED, false, 1, false>;
   } else {
-    fn = interleaved ? (const void*)rotary_kernel<T, V, ALIGNED, true> : (const void*)rotary_kernel<T, V, ALIGNED, false>;
+    fn = interleaved ? (pack ? (const void*)rotary_kernel<T, V, CV, ALIGNED, true, 2, true> : (const void*)rotary_kernel<T, V, CV, ALIGNED, true, 1, false>)
+                     : (pack ? (const void*)rotary_kernel<T, V, CV, ALIGNED, false, 2, true> : (const void*)rotary_kernel<T, V, CV, ALIGNED, false, 1, false>);
   }
   void* params[] = {&a};
   const size_t smem = sizeof(float2) * kRotTokens * static_cast<size_t>(a.pairs);
@@ -203,35 +233,35 @@ static int rot_launch_v(RotArgs& a, bool interleaved, cudaStream_t st) {
   return ND_OK;
 }
 
-template <typename T> static int rot_launch(RotArgs& a, bool interleaved, cudaStream_t st) {
+template <typename T> static int rot_launch(RotArgs& a, bool interleaved, bool pack, cudaStream_t st) {
   // the widest vector that divides every offset a slot can have and every base address: 16 bytes where R (half layout)
-  // or 2 R (interleaved) allow it; half of 72 dimensions is 36, which makes it 8 bytes for 16-bit types
-  unsigned long long mix = static_cast<unsigned long long>(a.head_dim) | (2ull * a.pairs);
-  if (!interleaved) mix |= static_cast<unsigned long long>(a.pairs);
-  unsigned long long addr = 0;
-  for (int g = 0; g < a.n_seg; ++g) {
+  // or 2 R (interleaved) allow it; half of 72 dimensions is 36, which makes it 8 bytes for 16-bit types (v keeps 16)
+  unsigned long long mix = static_cast<unsigned long long>(a.head_dim), addr = 0;
+  for (int g = 0; g < (pack ? 3 : 1); ++g) {
     const RotSeg& s = a.seg[g];
     mix |= static_cast<unsigned long long>(s.src_h) | static_cast<unsigned long long>(s.src_s) |
            static_cast<unsigned long long>(s.src_b) | static_cast<unsigned long long>(s.dst_h) |
            static_cast<unsigned long long>(s.dst_s) | static_cast<unsigned long long>(s.dst_b);
     addr |= reinterpret_cast<uintptr_t>(s.src) | reinterpret_cast<uintptr_t>(s.dst);
   }
-  auto fits = [&](unsigned v) { return mix % v == 0 && addr % (v * sizeof(T)) == 0; };
+  const unsigned long long rot = mix | (2ull * a.pairs) | (interleaved ? 0ull : static_cast<unsigned long long>(a.pairs));
+  auto fits = [&](unsigned long long what, unsigned v) { return what % v == 0 && addr % (v * sizeof(T)) == 0; };
+  constexpr int kWide = 16 / sizeof(T);
+  if (fits(rot, kWide)) return rot_launch_v<T, kWide, kWide, true>(a, interleaved, pack, st);
   if constexpr (sizeof(T) == 2) {
-    if (fits(8)) return rot_launch_v<T, 8, true>(a, interleaved, st);
+    if (fits(rot, 4)) return fits(mix, 8) ? rot_launch_v<T, 4, 8, true>(a, interleaved, pack, st) : rot_launch_v<T, 4, 4, true>(a, interleaved, pack, st);
   }
-  if (fits(4)) return rot_launch_v<T, 4, true>(a, interleaved, st);
-  if (fits(2)) return rot_launch_v<T, 2, true>(a, interleaved, st);
+  if (fits(rot, 2)) return rot_launch_v<T, 2, 2, true>(a, interleaved, pack, st);
   // odd head dimensions, odd strides or odd addresses: single elements (adjacent pairs as two of them, where the rest
   // of the head is even too)
-  if (!interleaved) return rot_launch_v<T, 1, true>(a, false, st);
-  if (a.head_dim % 2 == 0) return rot_launch_v<T, 2, false>(a, true, st);
+  if (!interleaved) return rot_launch_v<T, 1, 1, true>(a, false, pack, st);
+  if (a.head_dim % 2 == 0) return rot_launch_v<T, 2, 2, false>(a, true, pack, st);
   return ND_ERR_UNSUPPORTED;
 }
 
 static int rot_entry(int dtype, RotArgs& a, int64_t batch, int64_t seq_len, int64_t heads, int64_t head_dim,
                      const void* positions, int pos_bytes, int64_t pos_stride_b, const double* freqs, int64_t pairs,
-                     int64_t axes, int interleaved, float factor, int inverse, void* stream) {
+                     int64_t axes, int interleaved, float factor, int inverse, bool pack, void* stream) {
   a.positions = positions; a.freqs = freqs;
   a.tokens = batch * seq_len; a.seq_len = seq_len; a.pos_b = pos_stride_b;
   a.heads = static_cast<int>(heads); a.head_dim = static_cast<int>(head_dim);
@@ -239,9 +269,9 @@ static int rot_entry(int dtype, RotArgs& a, int64_t batch, int64_t seq_len, int6
   a.factor = factor; a.inverse = inverse;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case ND_F16: return rot_launch<__half>(a, interleaved != 0, st);
-    case ND_BF16: return rot_launch<__nv_bfloat16>(a, interleaved != 0, st);
-    case ND_F32: return rot_launch<float>(a, interleaved != 0, st);
+    case ND_F16: return rot_launch<__half>(a, interleaved != 0, pack, st);
+    case ND_BF16: return rot_launch<__nv_bfloat16>(a, interleaved != 0, pack, st);
+    case ND_F32: return rot_launch<float>(a, interleaved != 0, pack, st);
     default: return ND_ERR_UNSUPPORTED;
   }
 }
@@ -272,10 +302,9 @@ int nd_rotary(int dtype, const void* x, void* y, int64_t batch, int64_t seq_len,
   if (batch == 0 || seq_len == 0) return ND_OK;
   if (!x || !y || !positions || !freqs) return ND_ERR_BAD_ARG;
   RotArgs a{};
-  a.n_seg = 1;
-  a.seg[0] = RotSeg{x, y, stride_b, stride_s, stride_h, seq_len * heads * head_dim, heads * head_dim, head_dim, 1};
+  a.seg[0] = RotSeg{x, y, stride_b, stride_s, stride_h, seq_len * heads * head_dim, heads * head_dim, head_dim};
   return rot_entry(dtype, a, batch, seq_len, heads, head_dim, positions, pos_bytes, pos_stride_b, freqs, pairs, axes,
-                   interleaved, factor, inverse, stream);
+                   interleaved, factor, inverse, false, stream);
 }
 
 static int qkv_rotary(bool pack, int dtype, const void* qkv, const void* const* part, int64_t batch, int64_t seq_len,
@@ -289,15 +318,14 @@ static int qkv_rotary(bool pack, int dtype, const void* qkv, const void* const* 
   const int64_t hidden = heads * head_dim;
   const size_t es = dtype == ND_F32 ? 4 : 2;
   RotArgs a{};
-  a.n_seg = 3;
   for (int g = 0; g < 3; ++g) {
     void* wide = const_cast<char*>(static_cast<const char*>(qkv)) + g * hidden * es;
     void* narrow = const_cast<void*>(part[g]);
-    a.seg[g] = pack ? RotSeg{wide, narrow, seq_len * 3 * hidden, 3 * hidden, head_dim, seq_len * hidden, hidden, head_dim, g < 2}
-                    : RotSeg{narrow, wide, seq_len * hidden, hidden, head_dim, seq_len * 3 * hidden, 3 * hidden, head_dim, g < 2};
+    a.seg[g] = pack ? RotSeg{wide, narrow, seq_len * 3 * hidden, 3 * hidden, head_dim, seq_len * hidden, hidden, head_dim}
+                    : RotSeg{narrow, wide, seq_len * hidden, hidden, head_dim, seq_len * 3 * hidden, 3 * hidden, head_dim};
   }
   return rot_entry(dtype, a, batch, seq_len, heads, head_dim, positions, pos_bytes, pos_stride_b, freqs, pairs, axes,
-                   interleaved, factor, pack ? 0 : 1, stream);
+                   interleaved, factor, pack ? 0 : 1, true, stream);
 }
 
 int nd_qkv_pack_rotary_fwd(int dtype, const void* qkv, void* q, void* k, void* v, int64_t batch, int64_t seq_len,

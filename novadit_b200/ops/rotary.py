@@ -106,6 +106,9 @@ def fused_rotary(x, positions, freqs, interleaved: bool = False, attention_facto
     `attention_factor`. Interleaved pairs need an even D. Differentiable in x."""
     require_cuda_extension("fused_rotary", x, "rotary_ref")
     _check_even(x.shape[-1], interleaved)
+    if not (torch.is_grad_enabled() and x.requires_grad):  # nothing to record
+        ext = require_cuda_extension("fused_rotary", x, "rotary_ref")
+        return ext.fused_rotary_apply(x, positions, freqs, bool(interleaved), float(attention_factor), False)
     return _FusedRotaryFunction.apply(x, positions, freqs, bool(interleaved), float(attention_factor))
 
 
@@ -134,6 +137,10 @@ def fused_qkv_pack_rotary(qkv, num_heads: int, head_dim: int, positions, freqs, 
         raise ValueError(f"Expected last dim {3 * num_heads * head_dim}, got {tuple(qkv.shape)}")
     require_cuda_extension("fused_qkv_pack_rotary", qkv, "qkv_pack_rotary_ref")
     _check_even(head_dim, interleaved)
+    if not (torch.is_grad_enabled() and qkv.requires_grad):  # nothing to record
+        ext = require_cuda_extension("fused_qkv_pack_rotary", qkv, "qkv_pack_rotary_ref")
+        return tuple(ext.fused_qkv_pack_rotary_forward(qkv, num_heads, head_dim, positions, freqs, bool(interleaved),
+                                                       float(attention_factor)))
     return _FusedQkvPackRotaryFunction.apply(qkv, num_heads, head_dim, positions, freqs, bool(interleaved),
                                              float(attention_factor))
 
