@@ -7,8 +7,8 @@
 // becomes a 64-bit fixed-point fraction of a turn, and position * fraction is ONE 64-bit integer product whose overflow
 // drops the whole turns: the remainder is exact, whatever the position. Its top 32 bits go to sincospi.
 //
-// Bound: HBM, one read and one write of every element (plus one position per token and axis). A CTA takes kRotTokens
-// tokens and fills a table of kRotTokens x R (cos, sin) in shared memory once; all heads of q and k read it, so a sine costs
+// Bound: HBM, one read and one write of every element (plus one position per token and axis). A CTA takes two or
+// four tokens and fills a table of (cos, sin) for them in shared memory once; all heads of q and k read it, so a sine costs
 // the kernel 1 / heads of what it would cost per element. A thread owns one vector slot of the token (a pair of vectors R
 // apart in the half layout, one vector of adjacent pairs in the interleaved one, a plain copy elsewhere), of q and of k
 // alike, and one 16-byte slot of v. The loads of its first slots, of all the CTA's tokens, are issued before the table is
@@ -18,8 +18,10 @@
 namespace nd {
 
 constexpr int kRotThreads = 256;
-constexpr int kRotTokens = 4;       // tokens per CTA
-constexpr int kRotMaxPairs = 1024;  // table of kRotTokens * pairs * 8 bytes = 32 KB at most
+constexpr int kRotMaxPairs = 1024;  // table of at most 4 tokens * pairs * 8 bytes = 32 KB
+// Tokens per CTA: two where a thread has q, k and v of each (8 x 4096 x 3 x 16 x 72 bf16: 83 us, with four 90, whose registers
+// leave three CTAs on an SM), four of one tensor (30021 x 12 x 64 fp32: 31 us, with two 35)
+template <int ROT> constexpr int rot_tokens = ROT == 2 ? 2 : 4;
 
 struct RotSeg {  // one tensor of [tokens, heads, D]; strides in elements
   const void* src;
@@ -70,6 +72,7 @@ __device__ __forceinline__ int rot_div(int n, unsigned mul) {
 // ROT rotated segments (x, or q and k), COPY: a copied one behind them (v), in vectors of CV elements
 template <typename T, int V, int CV, bool ALIGNED, bool INTERLEAVED, int ROT, bool COPY>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(const RotArgs a) {
+  constexpr int kRotTokens = rot_tokens<ROT>;
   extern __shared__ float2 table[];  // [kRotTokens][pairs]
   constexpr int kParts = INTERLEAVED ? 1 : 2;  // vectors per rotated slot
   const long long t0 = static_cast<long long>(blockIdx.x) * kRotTokens;
@@ -210,7 +213,8 @@ static int rot_launch_v(RotArgs& a, bool interleaved, bool pack, cudaStream_t st
   a.copy_mul = rot_mul(a.copy_units);
   const long long all = static_cast<long long>(a.heads) * (a.units > a.copy_units ? a.units : a.copy_units);
   if (all >= 65536) return ND_ERR_UNSUPPORTED;  // rot_div's range
-  const long long grid = (a.tokens + kRotTokens - 1) / kRotTokens;
+  const int per_cta = pack ? rot_tokens<2> : rot_tokens<1>;
+  const long long grid = (a.tokens + per_cta - 1) / per_cta;
   if (grid > 0x7FFFFFFFLL) return ND_ERR_UNSUPPORTED;
   const int slots = a.heads * a.units;
   const int passes = (slots + kRotThreads - 1) / kRotThreads;
@@ -223,7 +227,7 @@ static int rot_launch_v(RotArgs& a, bool interleaved, bool pack, cudaStream_t st
                      : (pack ? (const void*)rotary_kernel<T, V, CV, ALIGNED, false, 2, true> : (const void*)rotary_kernel<T, V, CV, ALIGNED, false, 1, false>);
   }
   void* params[] = {&a};
-  const size_t smem = sizeof(float2) * kRotTokens * static_cast<size_t>(a.pairs);
+  const size_t smem = sizeof(float2) * per_cta * static_cast<size_t>(a.pairs);
   cudaError_t e = cudaLaunchKernel(fn, dim3(static_cast<unsigned>(grid)), dim3(nt), params, smem, st);
   if (e != cudaSuccess) {
     set_last_cuda_error(e);
