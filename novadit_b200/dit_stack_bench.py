@@ -2,6 +2,7 @@
 the PyTorch definitions of the same stack.
 
     python -m novadit_b200.dit_stack_bench [--depth 28 --batch 32 --seq 256 --hidden 1152 --heads 16]
+    python -m novadit_b200.dit_stack_bench --rotary --context 77      # rotary positions, cross attention to a prompt
     python -m torch.distributed.run --nproc-per-node N ... -m novadit_b200.dit_stack_bench   # one batch per GPU
 
 Latent [B, S, H] ~ N(0, 1), conditioning [B, H] ~ N(0, 1), weights N(0, 0.02) from a seeded CPU generator, bf16;
@@ -45,6 +46,9 @@ def main() -> None:
     ap.add_argument("--iters", type=int, default=5)
     ap.add_argument("--warmup", type=int, default=2)
     ap.add_argument("--no-ref", action="store_true", help="skip the PyTorch-definition stack")
+    ap.add_argument("--rotary", action="store_true", help="rotary positions (row and column) in the self attention")
+    ap.add_argument("--context", type=int, default=0, help="prompt tokens every block reads by cross attention (0: none)")
+    ap.add_argument("--context-size", type=int, default=1024, help="width of the prompt's states")
     ap.add_argument("--zero-init", action="store_true", help="adaLN-Zero initialisation (blocks are identities)")
     args = ap.parse_args()
 
@@ -68,14 +72,24 @@ def main() -> None:
     cond = torch.randn(args.batch, args.hidden, generator=gen).to(dev, dt).requires_grad_(True)
     dy = torch.randn(args.batch, args.seq, args.hidden, generator=gen).to(dev, dt)
 
+    side = max(1, int(args.seq ** 0.5))
+    where = torch.arange(args.seq, device=dev)
+    positions = torch.stack([where // side, where % side], dim=-1) if args.rotary else None
+    context = lens = None
+    if args.context:
+        context = torch.randn(args.batch, args.context, args.context_size, generator=gen).to(dev, dt)
+        lens = torch.randint(0, args.context + 1, (args.batch,), generator=gen, dtype=torch.int32).to(dev)
+
     def build(fused: bool):
         stack = DiTStack(args.hidden, args.heads, args.depth, use_fused=fused, zero_init=args.zero_init,
-                         device=dev, dtype=dt)
+                         device=dev, dtype=dt, rotary_axes=2 if args.rotary else 0,
+                         context_size=args.context_size if args.context else None)
         init_stack_(stack, seed=0, zero_init=args.zero_init)
-        targets = (x, cond, *stack.parameters())
+        # (with rotary positions the reference's own attention has no part in the result)
+        targets = (x, cond, *(p for n, p in stack.named_parameters() if not (args.rotary and ".body.attn." in n)))
 
         def step():
-            y = stack(x, cond)
+            y = stack(x, cond, positions, context, lens)
             return y, torch.autograd.grad(y, targets, dy)
 
         return stack, step
@@ -83,6 +97,8 @@ def main() -> None:
     result = {"workload": f"config5: DiT stack depth {args.depth}, H {args.hidden}, {args.heads} heads, "
                           f"x [{args.batch},{args.seq},{args.hidden}] bf16 per GPU, fwd+bwd",
               "n_gpus": world, "data": "synthetic"}
+    if args.rotary or args.context:
+        result["workload"] += f", rotary {args.rotary}, prompt {args.context} x {args.context_size}"
     _, fused_step = build(True)
     fused_ms = statistics.median(time_steps(fused_step, args.warmup, args.iters))
     yf, gf = fused_step()

@@ -85,12 +85,71 @@ class _FusedFc1MLP(nn.Module):
         return m.fc2(ops.fused_fc1_bias_act(x, m.fc1.weight, m.fc1.bias, m.activation))
 
 
+class RotaryAttention(nn.Module):
+    """Self attention of a DiT block with rotary positions: the fused projection is split and rotated in one pass
+    (`ops.fused_qkv_pack_rotary`), attended (`ops.fused_cross_attention`, queries and keys of one sequence) and projected.
+    `axes` position axes (2 for images: row and column of the patch) share the head's dimensions evenly; `positions` is
+    [S, axes] or [B, S, axes] ([S] or [B, S] with one axis). `use_fused=False` evaluates the PyTorch definitions."""
+
+    def __init__(self, hidden_size: int, num_heads: int, axes: int = 2, base: float = 10000.0, use_fused: bool = True,
+                 device=None, dtype=None) -> None:
+        super().__init__()
+        if hidden_size % num_heads != 0:
+            raise ValueError(f"hidden_size must be a multiple of num_heads, got {hidden_size} and {num_heads}")
+        self.num_heads, self.head_dim, self.use_fused = num_heads, hidden_size // num_heads, use_fused
+        self.qkv = nn.Linear(hidden_size, 3 * hidden_size, device=device, dtype=dtype)
+        self.proj = nn.Linear(hidden_size, hidden_size, device=device, dtype=dtype)
+        rotary_dim = self.head_dim // (2 * axes) * (2 * axes)
+        freqs, _ = ops.rotary_frequencies(rotary_dim, base, axes, device=device)
+        self.register_buffer("freqs", freqs, persistent=False)
+
+    def _apply(self, fn, recurse=True):  # a module moved to another dtype keeps its frequencies in 64 bits
+        freqs = self.freqs
+        super()._apply(fn, recurse)
+        self.freqs = freqs.to(self.freqs.device)
+        return self
+
+    def forward(self, x: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
+        pack = ops.fused_qkv_pack_rotary if self.use_fused else ops.qkv_pack_rotary_ref
+        attend = ops.fused_cross_attention if self.use_fused else ops.cross_attention_ref
+        q, k, v = pack(self.qkv(x), self.num_heads, self.head_dim, positions, self.freqs)
+        return self.proj(attend(q, k, v).flatten(2))
+
+
+class CrossAttention(nn.Module):
+    """Attention of the latent tokens to the states of a prompt [B, M, context_size], padded: `context_mask` [B, M] bool or
+    `context_lens` [B]. Keys and values come from one projection and are attended where they lie; a sample with an
+    empty prompt gets the projection's bias. `use_fused=False` evaluates the PyTorch definition."""
+
+    def __init__(self, hidden_size: int, context_size: int, num_heads: int, num_kv_heads: int | None = None,
+                 use_fused: bool = True, device=None, dtype=None) -> None:
+        super().__init__()
+        kv_heads = num_heads if num_kv_heads is None else num_kv_heads
+        if hidden_size % num_heads != 0 or num_heads % kv_heads != 0:
+            raise ValueError("hidden_size must be a multiple of num_heads and num_heads of num_kv_heads, got "
+                             f"{hidden_size}, {num_heads} and {kv_heads}")
+        self.num_heads, self.kv_heads, self.head_dim = num_heads, kv_heads, hidden_size // num_heads
+        self.use_fused = use_fused
+        self.q = nn.Linear(hidden_size, hidden_size, device=device, dtype=dtype)
+        self.kv = nn.Linear(context_size, 2 * kv_heads * self.head_dim, device=device, dtype=dtype)
+        self.proj = nn.Linear(hidden_size, hidden_size, device=device, dtype=dtype)
+
+    def forward(self, x: torch.Tensor, context: torch.Tensor, context_mask=None, context_lens=None) -> torch.Tensor:
+        q = self.q(x).unflatten(2, (self.num_heads, self.head_dim))
+        k, v = self.kv(context).unflatten(2, (2, self.kv_heads, self.head_dim)).unbind(2)
+        attend = ops.fused_cross_attention if self.use_fused else ops.cross_attention_ref
+        return self.proj(attend(q, k, v, key_mask=context_mask, kv_lens=context_lens).flatten(2))
+
+
 class AdaLNZeroBlock(nn.Module):
-    """One DiT block with adaLN-Zero conditioning around the parts of an unchanged reference `NovaDiTBlock`."""
+    """One DiT block with adaLN-Zero conditioning around the parts of an unchanged reference `NovaDiTBlock`.
+
+    `rotary_axes` > 0 replaces the reference's attention, which has no positions, by `RotaryAttention`; `context_size`
+    adds `CrossAttention` to a prompt between the attention and the MLP branch, on the residual stream without gate."""
 
     def __init__(self, hidden_size: int, num_heads: int, mlp_ratio: float = 4.0, use_fused: bool = True,
                  use_fused_fc1_bias_act: bool = True, activation: str = "gelu", zero_init: bool = True,
-                 device=None, dtype=None) -> None:
+                 device=None, dtype=None, rotary_axes: int = 0, context_size: int | None = None) -> None:
         super().__init__()
         ref = reference_modules()
         self.use_fused = use_fused
@@ -109,12 +168,22 @@ class AdaLNZeroBlock(nn.Module):
         if zero_init:
             nn.init.zeros_(self.modulation.weight)
             nn.init.zeros_(self.modulation.bias)
+        self.rotary_attn = (RotaryAttention(hidden_size, num_heads, rotary_axes, use_fused=use_fused, device=device, dtype=dtype)
+                            if rotary_axes > 0 else None)
+        self.cross_attn = (CrossAttention(hidden_size, context_size, num_heads, use_fused=use_fused, device=device, dtype=dtype)
+                           if context_size is not None else None)
 
-    def forward(self, x: torch.Tensor, cond: torch.Tensor) -> torch.Tensor:
+    def attend(self, h: torch.Tensor, positions=None) -> torch.Tensor:
+        return self.body.attn(h) if self.rotary_attn is None else self.rotary_attn(h, positions)
+
+    def forward(self, x: torch.Tensor, cond: torch.Tensor, positions=None, context=None, context_lens=None) -> torch.Tensor:
         shift_a, scale_a, gate_a, shift_m, scale_m, gate_m = self.modulation(F.silu(cond)).chunk(6, dim=-1)
         body = self.body
         residual = ops.fused_gated_residual if self.use_fused else ops.gated_residual_ref
-        x = residual(x, body.attn(body._adaln(x, scale_a.contiguous(), shift_a.contiguous())), gate_a)
+        x = residual(x, self.attend(body._adaln(x, scale_a.contiguous(), shift_a.contiguous()), positions), gate_a)
+        if self.cross_attn is not None:
+            plain = ops.fused_out_residual if self.use_fused else ops.out_residual_ref
+            x = plain(x, self.cross_attn(x, context, context_lens=context_lens))
         x = residual(x, self.mlp_branch(body._adaln(x, scale_m.contiguous(), shift_m.contiguous())), gate_m)
         return x
 
@@ -126,18 +195,21 @@ class DiTStack(nn.Module):
 
     def __init__(self, hidden_size: int = 1152, num_heads: int = 16, depth: int = 28, mlp_ratio: float = 4.0,
                  use_fused: bool = True, use_fused_fc1_bias_act: bool = True, activation: str = "gelu",
-                 zero_init: bool = True, device=None, dtype=None) -> None:
+                 zero_init: bool = True, device=None, dtype=None, rotary_axes: int = 0,
+                 context_size: int | None = None) -> None:
         super().__init__()
         self.blocks = nn.ModuleList([
             AdaLNZeroBlock(hidden_size, num_heads, mlp_ratio, use_fused, use_fused_fc1_bias_act, activation,
-                           zero_init, device, dtype)
+                           zero_init, device, dtype, rotary_axes, context_size)
             for _ in range(depth)
         ])
 
-    def forward(self, x: torch.Tensor, cond: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, cond: torch.Tensor, positions=None, context=None, context_lens=None) -> torch.Tensor:
+        """`positions` for blocks with rotary axes; `context` [B, M, context_size] and `context_lens` [B] (None: no
+        padding) for blocks that read a prompt."""
         if not (self.blocks and self.blocks[0].use_fused):
             for block in self.blocks:
-                x = block(x, cond)
+                x = block(x, cond, positions, context, context_lens)
             return x
         # Fused stack: the gated residual of a branch and the AdaLN of the NEXT branch are one kernel
         # (`ops.fused_residual_adaln`), also across block boundaries, so a block's MLP residual is applied by the
@@ -152,7 +224,11 @@ class DiTStack(nn.Module):
                 h = body._adaln(x, scale_a.contiguous(), shift_a.contiguous())
             else:
                 x, h = ops.fused_residual_adaln(x, pending[0], pending[1], scale_a.contiguous(), shift_a.contiguous())
-            x, h = ops.fused_residual_adaln(x, body.attn(h), gate_a, scale_m.contiguous(), shift_m.contiguous())
+            branch, gate = block.attend(h, positions), gate_a
+            if block.cross_attn is not None:  # it reads the stream: the attention's residual first, its own without a gate
+                x = ops.fused_gated_residual(x, branch, gate)
+                branch, gate = block.cross_attn(x, context, context_lens=context_lens), None
+            x, h = ops.fused_residual_adaln(x, branch, gate, scale_m.contiguous(), shift_m.contiguous())
             pending = (block.mlp_branch(h), gate_m)
         return ops.fused_gated_residual(x, pending[0], pending[1])
 
