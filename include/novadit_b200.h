@@ -49,7 +49,8 @@ int nd_last_cuda_error(void);
 int nd_version(void);
 /* Error word of the current device: 0, or the code a kernel left when one of its bounded waits
  * expired (1..3: a norm kernel waiting for a bulk copy into shared memory; 101..114: an FC1 kernel
- * waiting for an operand stage, an accumulator or a dy block - its output is then incomplete).
+ * waiting for an operand stage, an accumulator or a dy block; 201..256: an attention kernel waiting for a tile, a
+ * product or the other half of a row - its output is then incomplete).
  * Covers every kernel of the library, including launches made through the torch extension, which
  * passes no status word of its own. Synchronises with the device (a blocking copy).
  * reset != 0 clears it. Negative = nd_status of a failed query. */

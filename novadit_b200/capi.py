@@ -514,3 +514,39 @@ def rotary(x, positions, freqs, *, interleaved=False, factor=1.0, inverse=False,
                           positions.element_size(), 0 if shared else s * axes, _ptr(freqs), freqs.numel(), axes,
                           int(interleaved), factor, int(inverse), _stream()), "rotary")
     return y
+
+
+# ---------------------------------------------------------------- attention to keys of another length
+def _attn_strides(*ts):
+    flat = [n for t in ts for n in t.stride()[:3]]
+    return (c_int64 * len(flat))(*flat)
+
+
+def attn_fwd(q, k, v, *, key_mask=None, kv_lens=None, scale=None, with_lse=False):
+    """`nd_attn_fwd` on contiguous q [B, Sq, heads, D], k / v [B, Sk, kv_heads, D]; key_mask uint8 / bool [B, Sk] or
+    kv_lens int32 [B] -> (out, lse or None)."""
+    _need_cuda(q, k, v, key_mask, kv_lens)
+    b, sq, hq, d = q.shape
+    sk, hkv = k.shape[1], k.shape[2]
+    out = torch.empty_like(q)
+    lse = torch.empty(lib().nd_attn_lse_floats(b, sq, hq, hkv), dtype=torch.float32, device=q.device) if with_lse else None
+    nbytes = lib().nd_attn_fwd_ws_bytes(b, sq, sk, hq, hkv, d)
+    ws = _WS.get(nbytes, q.device, _stream())
+    check(lib().nd_attn_fwd(DTYPE_IDS[q.dtype], _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(key_mask), _ptr(kv_lens),
+                            b, sq, sk, hq, hkv, d, _attn_strides(q, k, v), d ** -0.5 if scale is None else scale, _ptr(ws),
+                            nbytes, _stream()), "attn_fwd")
+    return out, lse
+
+
+def attn_bwd(dout, q, k, v, out, lse, *, key_mask=None, kv_lens=None, scale=None):
+    """`nd_attn_bwd` -> (dq, dk, dv)."""
+    _need_cuda(dout, q, k, v, out, lse, key_mask, kv_lens)
+    b, sq, hq, d = q.shape
+    sk, hkv = k.shape[1], k.shape[2]
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    nbytes = lib().nd_attn_bwd_ws_bytes(b, sq, sk, hq, hkv, d)
+    ws = _WS.get(nbytes, q.device, _stream())
+    check(lib().nd_attn_bwd(DTYPE_IDS[q.dtype], _ptr(dout), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(dq), _ptr(dk),
+                            _ptr(dv), _ptr(key_mask), _ptr(kv_lens), b, sq, sk, hq, hkv, d, _attn_strides(q, k, v, dout),
+                            d ** -0.5 if scale is None else scale, _ptr(ws), nbytes, _stream()), "attn_bwd")
+    return dq, dk, dv

@@ -52,7 +52,10 @@ template <int NB> struct __align__(1024) BwdSmem {
   // where the second was
   uint8_t out[4][(NB == 1 ? 2 : 3) * kStageBytes];
   int lens[kLens];
-  alignas(16) float stat[kRing / 2][2][kTile];  // dK/dV: log-sum-exp and delta of the query tile
+  union {
+    alignas(16) float stat[kRing / 2][2][kTile];  // dK/dV: log-sum-exp and delta of the query tile
+    float2 red[2][4][kTile];                      // dQ: [exchange parity][warpgroup][row]
+  };
   uint64_t res_full, res_empty;
   uint64_t full[kRing], empty[kRing];
   uint64_t s_full[2], dp_full[2];   // MMA -> elementwise, per half
@@ -61,7 +64,6 @@ template <int NB> struct __align__(1024) BwdSmem {
   uint64_t acc_done;                // the accumulators are complete
   uint64_t o_read;                  // dQ: the elementwise warps have read dO and O
   uint64_t swap[4];                 // dQ: the four warps of 32 rows have written to `red`
-  float red[2][4][kTile];           // dQ: [exchange parity][warpgroup][row]
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -313,14 +315,15 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     uint32_t items = 0;
     int it = 0;
     bool ok = true;
-    // sum over the four threads of a row, once per item
-    auto exchange = [&](float v, float& sum) -> bool {
+    // sums over the four threads of a row, once per item
+    auto exchange = [&](float2 v, float2& sum) -> bool {
       s.red[items & 1][group][r] = v;
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.swap[quarter]);
       if (!warp_wait(&s.swap[quarter], items & 1, abort_flag, a.sink, 139)) return false;
-      const float* red = s.red[items & 1][0] + r;
-      sum = (red[0] + red[kTile]) + (red[2 * kTile] + red[3 * kTile]);
+      const float2* red = s.red[items & 1][0] + r;
+      sum.x = (red[0].x + red[kTile].x) + (red[2 * kTile].x + red[3 * kTile].x);
+      sum.y = (red[0].y + red[kTile].y) + (red[2 * kTile].y + red[3 * kTile].y);
       return true;
     };
     for (int item = blockIdx.x; item < a.items && ok; item += gridDim.x) {
@@ -354,8 +357,10 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           if (lane == 0) mbar_arrive(&s.o_read);
         }
         if (w.o || (half == 1 && w.n1 == 0)) {  // (the second: nothing to add to the one tile's sum below)
-          ok = exchange(ndelta, ndelta);
+          float2 sum;
+          ok = exchange(make_float2(ndelta, 0.f), sum);
           if (!ok) break;
+          ndelta = sum.x;
         }
       }
       const float factor = kHalf ? grad_factor(peak) : 1.f;
@@ -399,13 +404,18 @@ attn_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
           if (quarter == 0 && !((bits >> lane) & 1u)) clear_row<NB>(s.ring[k_at % kRing], group * 32 + lane);
           fence_proxy_async_smem();
         }
-        if (!w.o) {  // one key tile: delta = sum of P dP over the row's keys
-          uint64_t acc = 0;
+        if (!w.o) {  // one key tile: delta = sum of P dP over the row's keys, over the sum of P (1 but for its last bits)
+          uint64_t acc = 0, norm = 0;
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) acc = f2_fma(f2_pack(p[e], p[e + 1]), f2_pack(dp[e], dp[e + 1]), acc);
-          const float2 v = f2_unpack(acc);
-          ok = exchange(-(v.x + v.y), ndelta);
+          for (int e = 0; e < 32; e += 2) {
+            acc = f2_fma(f2_pack(p[e], p[e + 1]), f2_pack(dp[e], dp[e + 1]), acc);
+            norm = f2_add(norm, f2_pack(p[e], p[e + 1]));
+          }
+          const float2 v = f2_unpack(acc), n = f2_unpack(norm);
+          float2 sum;
+          ok = exchange(make_float2(v.x + v.y, n.x + n.y), sum);
           if (!ok) break;
+          ndelta = sum.y > 0.f ? -sum.x / sum.y : -sum.x;
         }
         uint32_t pk[16];
         const uint64_t nd2 = f2_pack(ndelta * factor, ndelta * factor), factor2 = f2_pack(factor, factor);

@@ -499,6 +499,7 @@ template <typename T> static const void* pick_fwd(int kt) {
 }
 
 int attn_launch(const void* fn, dim3 grid, int threads, size_t smem, void** params, cudaStream_t st) {
+  RelaxedCapture relaxed;  // the attribute and a first launch load the kernel's module
   if (smem > 0) {
     const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) {

@@ -25,6 +25,16 @@ inline int check_launch() {
   return ND_OK;
 }
 
+// Set-up that a first call needs (binding a context, loading a module, asking for a symbol's address) is not allowed on a
+// thread whose stream is being captured, unless the thread says that it may: a first call inside a capture then works.
+struct RelaxedCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  RelaxedCapture() { (void)cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~RelaxedCapture() { (void)cudaThreadExchangeStreamCaptureMode(&mode); }
+  RelaxedCapture(const RelaxedCapture&) = delete;
+  RelaxedCapture& operator=(const RelaxedCapture&) = delete;
+};
+
 int sm_count();  // multiprocessors of the current device (cached per device)
 int* device_error_ptr();  // device address of the error word kernels set when a bounded wait expires
 

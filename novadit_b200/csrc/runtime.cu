@@ -20,6 +20,7 @@ int* device_error_ptr() {
     return nullptr;
   }
   if (cache[dev] == nullptr) {
+    RelaxedCapture relaxed;
     void* p = nullptr;
     if (cudaGetSymbolAddress(&p, g_device_error) != cudaSuccess) {
       (void)cudaGetLastError();

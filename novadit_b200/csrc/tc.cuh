@@ -173,6 +173,7 @@ static EncodeTiledFn encode_fn() {
   // have none bound yet: one runtime call that needs the context binds the device's primary context to the thread.
   static thread_local bool context_bound = false;
   if (!context_bound) {
+    RelaxedCapture relaxed;
     (void)cudaFree(nullptr);
     context_bound = true;
   }

@@ -10,6 +10,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import require_cuda_extension
 
@@ -50,6 +51,7 @@ class _FusedCrossAttentionFunction(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         ext = require_cuda_extension("fused_cross_attention", dout, "cross_attention_ref")
         q, k, v, out, lse, key_mask, kv_lens = ctx.saved_tensors
@@ -65,7 +67,7 @@ def fused_cross_attention(q, k, v, key_mask=None, kv_lens=None, scale: float | N
     (the halves of a fused key/value projection, a transposed [B, heads, S, D]); others are copied. key_mask [B, Sk] bool
     (True: the key takes part) or kv_lens [B] int32 / int64 (the first kv_lens[b] keys, clamped to 0 .. Sk), not both;
     keys that take no part are never looked at. A sample without keys gives zeros and zero gradients. scale: 1 / sqrt(D)
-    by default, positive. Differentiable in q, k and v."""
+    by default, positive. Differentiable in q, k and v, once."""
     require_cuda_extension("fused_cross_attention", q, "cross_attention_ref")
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1]) if q.shape[-1] > 0 else 1.0

@@ -12,6 +12,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import require_cuda_extension
 from .qkv_pack import qkv_pack_ref
@@ -92,6 +93,7 @@ class _FusedRotaryFunction(torch.autograd.Function):
         return ext.fused_rotary_apply(x, positions, freqs, interleaved, attention_factor, False)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         ext = require_cuda_extension("fused_rotary", dy, "rotary_ref")
         positions, freqs = ctx.saved_tensors
@@ -103,7 +105,7 @@ def fused_rotary(x, positions, freqs, interleaved: bool = False, attention_facto
 
     positions int32 / int64 [S] or [B, S] with freqs float64 [R]; [S, axes] or [B, S, axes] with freqs [axes, R / axes]
     (`rotary_frequencies`). 2 R <= D: the dimensions behind are copied. The rotated part is multiplied by
-    `attention_factor`. Interleaved pairs need an even D. Differentiable in x."""
+    `attention_factor`. Interleaved pairs need an even D. Differentiable in x, once."""
     require_cuda_extension("fused_rotary", x, "rotary_ref")
     _check_even(x.shape[-1], interleaved)
     if not (torch.is_grad_enabled() and x.requires_grad):  # nothing to record
@@ -122,6 +124,7 @@ class _FusedQkvPackRotaryFunction(torch.autograd.Function):
                                                        attention_factor))
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk, dv):
         ext = require_cuda_extension("fused_qkv_pack_rotary", dq, "qkv_pack_rotary_ref")
         positions, freqs = ctx.saved_tensors
@@ -132,7 +135,7 @@ class _FusedQkvPackRotaryFunction(torch.autograd.Function):
 def fused_qkv_pack_rotary(qkv, num_heads: int, head_dim: int, positions, freqs, interleaved: bool = False,
                           attention_factor: float = 1.0):
     """`fused_qkv_pack` with `fused_rotary` of q and k in the same pass over qkv [B, S, 3 * heads * head_dim]: (q, k, v),
-    each [B, S, heads, head_dim] and contiguous. The other arguments as in `fused_rotary`. Differentiable in qkv."""
+    each [B, S, heads, head_dim] and contiguous. The other arguments as in `fused_rotary`. Differentiable in qkv, once."""
     if qkv.dim() != 3 or qkv.shape[-1] != 3 * num_heads * head_dim:
         raise ValueError(f"Expected last dim {3 * num_heads * head_dim}, got {tuple(qkv.shape)}")
     require_cuda_extension("fused_qkv_pack_rotary", qkv, "qkv_pack_rotary_ref")

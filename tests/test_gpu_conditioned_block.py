@@ -3,6 +3,10 @@ the same modules in 64 bits, and the adaLN-Zero block and stack around them. The
 stand-in with its interface gives the norm, the MLP and an attention."""
 from __future__ import annotations
 
+import os
+import subprocess
+import sys
+
 import pytest
 import torch
 import torch.nn.functional as F
@@ -168,3 +172,31 @@ def test_captured_step_beside_an_eager_one(stand_in):
     torch.cuda.synchronize()
     for a, b in zip(out, step()):
         assert rel_l2(a, b) < 1e-3  # (library products may choose other kernels while captured)
+
+
+FIRST_CALL = """
+import torch
+import novadit_b200.ops as ops
+qkv = torch.randn(2, 50, 3 * 288, device="cuda").bfloat16().requires_grad_(True)
+ctx = torch.randn(2, 20, 4, 72, device="cuda").bfloat16()
+pos, (freqs, _) = torch.arange(50, device="cuda"), ops.rotary_frequencies(72, device="cuda")
+dy = torch.randn(2, 50, 4, 72, device="cuda").bfloat16()
+def step():
+    q, k, v = ops.fused_qkv_pack_rotary(qkv, 4, 72, pos, freqs)
+    y = ops.fused_cross_attention(ops.fused_cross_attention(q, k, v), ctx, ctx)
+    return y.detach(), torch.autograd.grad(y, qkv, dy)[0]
+graph = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_may_be_captured():
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "same" in done.stdout, done.stderr[-2000:]

@@ -34,11 +34,12 @@ def make(b, n, m, h, hk, d, dtype, seed, fused=True):
     return q, k, v, dout
 
 
-def exact(q, k, v, dout, keep, scale):
+def exact(q, k, v, dout, keep, scale, tiny_s=None, tiny_p=None):
     """(out, dq, dk, dv) in 64 bits and their bars."""
     t = torch.finfo(q.dtype)
     e = t.eps / 2
     tiny = 0.0 if q.dtype == torch.bfloat16 else t.smallest_normal * t.eps / 2
+    tiny_s, tiny_p = (tiny if x is None else x for x in (tiny_s, tiny_p))
     b, n, h, d = q.shape
     m, hk = k.shape[1], k.shape[2]
     Q = q.detach().double().view(b, n, hk, h // hk, d).permute(0, 2, 3, 1, 4)
@@ -60,13 +61,13 @@ def exact(q, k, v, dout, keep, scale):
     ones = torch.ones_like(W)
     bar_o = e * O.abs() + (e + FINE) * WV + tiny * (ones @ V.abs()) + tiny
     dV = W.transpose(-1, -2) @ G
-    bar_v = (e + FINE) * (W.transpose(-1, -2) @ G.abs()) + tiny * (ones.transpose(-1, -2) @ G.abs())
+    bar_v = (e + FINE) * (W.transpose(-1, -2) @ G.abs()) + tiny_p * (ones.transpose(-1, -2) @ G.abs())
     dP = G @ V.transpose(-1, -2)
     delta = (G * O).sum(-1, keepdim=True)
     dS = W * (dP - delta)
     off = (G.abs() * (e * O.abs() + e * WV)).sum(-1, keepdim=True)  # delta's error
     mag = G.abs() @ V.abs().transpose(-1, -2) + (G.abs() * O.abs()).sum(-1, keepdim=True)
-    bar_s = e * dS.abs() + W * (off + FINE * mag) + tiny
+    bar_s = e * dS.abs() + W * (off + FINE * mag) + tiny_s
     dQ, dK = scale * (dS @ K), scale * (dS.transpose(-1, -2) @ Q)
     bar_q = scale * (bar_s @ K.abs())
     bar_k = scale * (bar_s.transpose(-1, -2) @ Q.abs())
@@ -318,6 +319,62 @@ def test_training_step_captured():
     graph.replay()
     torch.cuda.synchronize()
     assert not bool(out.any()) and not any(bool(g.any()) for g in grads)
+
+
+def test_one_key_takes_all_the_weight():
+    """Nothing a query does changes the result: its gradient, and the key's, are exactly zero; v's is the sum."""
+    for d, dtype in ((72, torch.bfloat16), (128, torch.float16)):
+        q, k, v, dout = make(3, 200, 9, 4, 2, d, dtype, 17)
+        out, dq, dk, dv = run(q, k, v, dout, kv_lens=torch.tensor([1, 1, 1], device=DEV))
+        assert torch.equal(out, v[:, :1].repeat_interleave(2, dim=2).expand(3, 200, 4, d))
+        assert not bool(dq.any()) and not bool(dk.any())
+
+
+@pytest.mark.parametrize("kind", ["lens32", "holes"])
+@pytest.mark.parametrize("b,n,m,h,hk,d", [(300, 20, 30, 2, 1, 64), (2, 9, 40000, 2, 2, 64), (300, 1, 30, 2, 2, 64), (70, 6, 1000, 2, 2, 72)])
+def test_many_samples_and_long_masks(kind, b, n, m, h, hk, d):
+    """More samples, or more mask, than the kernels keep key counts of."""
+    q, k, v, dout = make(b, n, m, h, hk, d, torch.bfloat16, 18)
+    key_mask, kv_lens, keep = masks(kind, b, m)
+    want, bars = exact(q, k, v, dout, keep, 1 / math.sqrt(d))
+    check(run(q, k, v, dout, key_mask=key_mask, kv_lens=kv_lens), want, bars)
+
+
+@pytest.mark.parametrize("size", [2.0 ** -10, 2.0 ** 11])
+@pytest.mark.parametrize("n,m", [(150, 90), (64, 700)])
+def test_gradients_of_other_magnitudes_in_fp16(size, n, m):
+    """dS of these would leave fp16's range (its normal numbers end at 6e-5, its largest at 65504) without the kernels' powers
+    of two: P is rounded times 2^floor(log2 m), dS times a power of two that brings the largest |dO| to 2^-4 or a little
+    below 2^-3, so half of fp16's smallest number, 2^-25, becomes 2^-25 / 2^floor(log2 m) and at most 2^-21 of that |dO|."""
+    q, k, v, dout = make(1, n, m, 2, 1, 64, torch.float16, 19)
+    dout = (dout.float() / 8 * size).half()
+    v = (v.float() * (8 if size > 1 else 1)).half()
+    want, bars = exact(q, k, v, dout, None, 0.125, 2.0 ** -21 * float(dout.abs().max()), 2.0 ** -25 / 2 ** int(math.log2(m)))
+    got = run(q, k, v, dout)
+    check(got, want, bars)
+    if size > 1:
+        assert float((want[1].abs().max())) < 6e4  # the gradients themselves fit
+
+
+def test_c_abi_helpers():
+    from novadit_b200 import capi
+
+    q, k, v, dout = make(2, 70, 90, 4, 2, 64, torch.float16, 20, fused=False)
+    lens = torch.tensor([90, 31], dtype=torch.int32, device=DEV)
+    want = run(q, k, v, dout, kv_lens=lens)
+    out, lse = capi.attn_fwd(q, k, v, kv_lens=lens, with_lse=True)
+    for a, b in zip((out, *capi.attn_bwd(dout, q, k, v, out, lse, kv_lens=lens)), want):
+        assert torch.equal(a, b)
+    keep = torch.arange(90, device=DEV)[None] < lens[:, None]
+    assert torch.equal(capi.attn_fwd(q, k, v, key_mask=keep)[0], out)
+
+
+def test_second_derivatives_are_refused():
+    q, k, v, dout = make(1, 8, 8, 1, 1, 16, torch.bfloat16, 21)
+    qd = q.detach().requires_grad_(True)
+    (dq,) = torch.autograd.grad(ops.fused_cross_attention(qd, k, v), qd, dout, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dq.float().sum(), qd)
 
 
 def test_refusals():
