@@ -3,13 +3,14 @@
 //
 // LPK lanes (the head's dimensions in 16-byte pieces, rounded up to a power of two) hold one key: its piece of K, then of
 // V, and the query rows' pieces in fp32. A score is 8 products per lane and a sum over the LPK lanes; every group of LPK
-// lanes ("slot") keeps its own running maximum, sum and output over the keys it sees, kUnroll of them at a time so that
-// 2 x kUnroll 16-byte loads are in flight per lane and the rescaling is paid once for all of them. Slots and warps are
+// lanes ("slot") keeps its own running maximum, sum and output over the keys it sees, kFewUnroll of them at a time so that
+// 2 x kFewUnroll 16-byte loads are in flight per lane and the rescaling is paid once for all of them. Slots and warps are
 // joined at the end. Weights are never rounded; everything is 32-bit until the output.
 //
 // A CTA takes (sample, key head, range of keys): the sample's own keys cut evenly into as many ranges as it takes to give
 // every SM several CTAs. More than one range: normalised partial outputs and their log-sum-exp go through the workspace
-// to a second kernel. Bound: HBM (K and V once).
+// to a second kernel. Bound: HBM (K and V once): 32 x 20 heads x
+// up to 1500 keys x 64, one token: 34 us, 0.56 of the copy rate; one query, one key: 6.4 us, the launch.
 #include "attn.cuh"
 
 namespace nd {

@@ -3,13 +3,14 @@
 // on a [B, S, heads, D] tensor, or on q and k while a fused projection [B, S, 3 heads D] is split into q, k, v (and on
 // the way back). The gradient is the same rotation by -t, so forward and backward share the kernel.
 //
-// The angle. t in radians as a 32-bit float is off by t * 2^-24, a tenth of a radian at position 10^6. Here a frequency
+// The angle. t in radians as a 32-bit float is off by t * 2^-24, 0.06 radians at position 10^6. Here a frequency
 // becomes a 64-bit fixed-point fraction of a turn, and position * fraction is ONE 64-bit integer product whose overflow
 // drops the whole turns: the remainder is exact, whatever the position. Its top 32 bits go to sincospi.
 //
 // Bound: HBM, one read and one write of every element (plus one position per token and axis). A CTA takes two or
 // four tokens and fills a table of (cos, sin) for them in shared memory once; all heads of q and k read it, so a sine costs
-// the kernel 1 / heads of what it would cost per element. A thread owns one vector slot of the token (a pair of vectors R
+// the kernel 1 / heads of what it would cost per element. 3 x 10007 x 12 x 64 fp32: 32 us, 5.8 TB/s, 0.88 of the copy rate;
+// pack of [32, 256, 3 x 16 x 72] bf16: 24.6 us, 4.6 TB/s; one token of eight sequences: 5.6 us, the launch. A thread owns one vector slot of the token (a pair of vectors R
 // apart in the half layout, one vector of adjacent pairs in the interleaved one, a plain copy elsewhere), of q and of k
 // alike, and one 16-byte slot of v. The loads of its first slots, of all the CTA's tokens, are issued before the table is
 // worked out and are in flight meanwhile: with the table first a CTA waits for memory four times in a row.
