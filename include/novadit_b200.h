@@ -268,15 +268,16 @@ int nd_qkv_pack_rotary_bwd(int dtype, const void* dq, const void* dk, const void
 /* -------------------------------------------------------------------- attention to keys of another length */
 
 /* out = softmax(scale * q k^T) v per sample and head, over the keys that take part.
- * q [batch, sq, hq, head_dim], k and v [batch, sk, hkv, head_dim] as strided views (`strides`: element strides of batch,
- * sequence and head for q, k, v: nine values, multiples of 8; head dimensions contiguous), out contiguous like q. Query
- * head h reads key head h / (hq / hkv). ND_F16 or ND_BF16, head_dim a multiple of 8 up to 128, bases 16-byte aligned,
- * anything else ND_ERR_UNSUPPORTED; scale positive and finite. Which keys take part (at most one of the two): key_mask
- * [batch, sk] bytes, non-zero = takes part; kv_lens [batch] ints, the first kv_lens[b] keys (values are clamped to
- * 0 .. sk). Others are never looked at: they may hold NaN. A sample without keys gives zeros. Scores, sums and outputs
- * are accumulated in fp32. `lse` (nullable; nd_attn_lse_floats values, 16-byte aligned, an order of its own) is what
- * the backward pass needs. `ws`: nd_attn_fwd_ws_bytes bytes, 16-byte aligned, no initialisation; 0 bytes unless there
- * is less work than SMs (then the keys are split over them and joined by a second small launch). It may be shared by
+ * q [batch, sq, hq, head_dim], k and v [batch, sk, hkv, head_dim] as strided views (`strides`: element strides of
+ * batch, sequence and head for q, k, v: nine values, multiples of 8, zero only for an extent of one; head dimensions
+ * contiguous), out contiguous like q. Query head h reads key head h / (hq / hkv). ND_F16 or ND_BF16, head_dim a
+ * multiple of 8 up to 128, bases 16-byte aligned, batch and heads up to 65535, sq up to 2^25, sk up to 2^30, anything
+ * else ND_ERR_UNSUPPORTED; scale positive and finite. Which keys take part (at most one of the two): key_mask [batch,
+ * sk] bytes, non-zero = takes part; kv_lens [batch] ints, the first kv_lens[b] keys (values are clamped to 0 .. sk).
+ * Others are never looked at: they may hold NaN. A sample without keys gives zeros. Scores, sums and outputs are
+ * accumulated in fp32. `lse` (nullable; nd_attn_lse_floats values, 16-byte aligned, an order of its own) is what the
+ * backward pass needs. `ws`: nd_attn_fwd_ws_bytes bytes, 16-byte aligned, no initialisation; 0 bytes unless there is
+ * less work than SMs (then the keys are split over them and joined by a second small launch). It may be shared by
  * launches on one stream, not by launches that may overlap. No counterpart in the reference, whose attention calls a
  * library (novadit/modules/dit_attention.py:10-80). */
 int64_t nd_attn_lse_floats(int64_t batch, int64_t sq, int64_t hq, int64_t hkv);

@@ -58,6 +58,15 @@ inline int attn_check(int dtype, int64_t b, int64_t sq, int64_t sk, int64_t hq, 
   return ND_OK;
 }
 
+// Element strides of a [B, S, H, ..] view: multiples of 16 bytes, and not zero where there is more than one element (a
+// tensor map walks no broadcast dimension)
+inline bool attn_strides_ok(const int64_t* st, int64_t b, int64_t s, int64_t h) {
+  const int64_t n[3] = {b, s, h};
+  for (int i = 0; i < 3; ++i)
+    if (st[i] < 0 || st[i] % 8 != 0 || (n[i] > 1 && st[i] == 0)) return false;
+  return true;
+}
+
 // [B, S, H, D] view with element strides -> boxes of `cols` columns x `heads` heads x `pos` positions
 static bool attn_map(CUtensorMap* map, int dtype, const void* base, int64_t b, int64_t s, int64_t h, int64_t d, int64_t sb,
                      int64_t ss, int64_t sh, int cols, int heads, int pos) {

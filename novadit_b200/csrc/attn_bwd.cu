@@ -874,8 +874,9 @@ int nd_attn_bwd(int dtype, const void* dout, const void* q, const void* k, const
   for (const void* p : {dout, q, k, v, out, static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv),
                         static_cast<const void*>(lse)})
     if (!aligned16(p)) return ND_ERR_UNSUPPORTED;
-  for (int i = 0; i < 12; ++i)
-    if (strides[i] < 0 || strides[i] % 8 != 0) return ND_ERR_UNSUPPORTED;
+  if (!attn_strides_ok(strides, batch, sq, hq) || !attn_strides_ok(strides + 3, batch, sk, hkv) ||
+      !attn_strides_ok(strides + 6, batch, sk, hkv) || !attn_strides_ok(strides + 9, batch, sq, hq))
+    return ND_ERR_UNSUPPORTED;
   if (ws == nullptr || ws_bytes < bwd_ws(a) || !aligned16(ws)) return ND_ERR_WORKSPACE;
   a.mask = AttnMask{static_cast<const unsigned char*>(key_mask), kv_lens};
   a.sink = WaitSink{nullptr, device_error_ptr()};

@@ -563,8 +563,9 @@ int nd_attn_fwd(int dtype, const void* q, const void* k, const void* v, void* ou
   a.s = attn_shape(batch, sq, sk, hq, hkv, head_dim);
   if (static_cast<long long>(a.s.sq) * a.s.gp > (1 << 30)) return ND_ERR_UNSUPPORTED;
   if (!aligned16(q) || !aligned16(out) || (sk > 0 && (!aligned16(k) || !aligned16(v)))) return ND_ERR_UNSUPPORTED;
-  for (int i = 0; i < 9; ++i)
-    if (strides[i] < 0 || strides[i] % 8 != 0) return ND_ERR_UNSUPPORTED;
+  if (!attn_strides_ok(strides, batch, sq, hq) || !attn_strides_ok(strides + 3, batch, sk, hkv) ||
+      !attn_strides_ok(strides + 6, batch, sk, hkv))
+    return ND_ERR_UNSUPPORTED;
   const AttnMask mask{static_cast<const unsigned char*>(key_mask), kv_lens};
   const float c = scale * 1.4426950408889634f;
   if (attn_few_takes(a.s)) {

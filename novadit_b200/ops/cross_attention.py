@@ -67,7 +67,7 @@ def fused_cross_attention(q, k, v, key_mask=None, kv_lens=None, scale: float | N
     (the halves of a fused key/value projection, a transposed [B, heads, S, D]); others are copied. key_mask [B, Sk] bool
     (True: the key takes part) or kv_lens [B] int32 / int64 (the first kv_lens[b] keys, clamped to 0 .. Sk), not both;
     keys that take no part are never looked at. A sample without keys gives zeros and zero gradients. scale: 1 / sqrt(D)
-    by default, positive. Differentiable in q, k and v, once."""
+    by default, positive. B and heads up to 65535. Differentiable in q, k and v, once."""
     require_cuda_extension("fused_cross_attention", q, "cross_attention_ref")
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1]) if q.shape[-1] > 0 else 1.0

@@ -45,6 +45,23 @@ def test_addresses_strides_and_workspace_are_checked():
     assert fwd(ptr=at, strides=nine, sq=100, sk=100000) == -4
 
 
+@pytest.mark.parametrize("tensor", [0, 1, 2, 3])
+@pytest.mark.parametrize("dim", [0, 1, 2])
+def test_broadcast_strides_are_refused_at_the_c_boundary(tensor, dim):
+    at = 1 << 20  # never looked at
+    L, p = capi.lib(), ctypes.c_void_p(1 << 20)
+    values = [8] * 12
+    values[3 * tensor + dim] = 0
+    twelve = (ctypes.c_int64 * 12)(*values)
+    many, one = (2, 100000, 100000, 4, 2), [2, 100000, 100000, 4, 2]  # b, sq, sk, hq, hkv
+    for i in {0: (0,), 1: (1, 2), 2: (3, 4)}[dim]:
+        one[i] = 1
+    if tensor < 3:
+        assert fwd(ptr=at, strides=twelve, b=many[0], sq=many[1], sk=many[2], hq=many[3], hkv=many[4]) == -2
+    for sizes, code in ((many, -2), (one, -4)):  # an extent of one has no stride; then the missing workspace is next
+        assert L.nd_attn_bwd(1, p, p, p, p, p, p, p, p, p, None, None, *sizes, 16, twelve, 0.25, None, 0, None) == code
+
+
 def test_workspace_sizes():
     L = capi.lib()
     assert L.nd_attn_lse_floats(2, 100, 8, 2) == 2 * 2 * 512  # blocks of four heads: 400 rows, padded to four tiles
