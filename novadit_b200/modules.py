@@ -99,12 +99,12 @@ class RotaryAttention(nn.Module):
         self.num_heads, self.head_dim, self.use_fused = num_heads, hidden_size // num_heads, use_fused
         self.qkv = nn.Linear(hidden_size, 3 * hidden_size, device=device, dtype=dtype)
         self.proj = nn.Linear(hidden_size, hidden_size, device=device, dtype=dtype)
-        rotary_dim = self.head_dim // (2 * axes) * (2 * axes)
-        freqs, _ = ops.rotary_frequencies(rotary_dim, base, axes, device=device)
-        self.register_buffer("freqs", freqs, persistent=False)
+        self.rotary = (self.head_dim // (2 * axes) * (2 * axes), base, axes)
+        self.register_buffer("freqs", ops.rotary_frequencies(*self.rotary, device=device)[0], persistent=False)
 
-    def _apply(self, fn, recurse=True):  # a module moved to another dtype keeps its frequencies in 64 bits
-        freqs = self.freqs
+    def _apply(self, fn, recurse=True):
+        # a module moved to another dtype keeps its frequencies in 64 bits; one that gets its memory now gets their values
+        freqs = ops.rotary_frequencies(*self.rotary)[0] if self.freqs.is_meta else self.freqs
         super()._apply(fn, recurse)
         self.freqs = freqs.to(self.freqs.device)
         return self

@@ -77,3 +77,14 @@ def test_cpu_tensors_are_refused():
         ops.fused_rotary(x, pos, f)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         ops.fused_qkv_pack_rotary(torch.zeros(1, 2, 24), 1, 8, pos, f)
+
+
+def test_attention_module_keeps_its_frequencies():
+    from novadit_b200.modules import RotaryAttention
+
+    want = ops.rotary_frequencies(16, 10000.0, 2)[0]
+    moved = RotaryAttention(64, 4, axes=2).to(torch.bfloat16)
+    placed = RotaryAttention(64, 4, axes=2, device="meta").to_empty(device="cpu")
+    for module in (moved, placed, placed.half()):
+        assert module.freqs.dtype == torch.float64 and torch.equal(module.freqs, want)
+    assert moved.qkv.weight.dtype == torch.bfloat16 and "freqs" not in moved.state_dict()
