@@ -10,7 +10,7 @@
 // A CTA takes (sample, key head, range of keys): the sample's own keys cut evenly into as many ranges as it takes to give
 // every SM several CTAs. More than one range: normalised partial outputs and their log-sum-exp go through the workspace
 // to a second kernel. Bound: HBM (K and V once): 32 x 20 heads x
-// up to 1500 keys x 64, one token: 34 us, 0.56 of the copy rate; one query, one key: 6.4 us, the launch.
+// up to 1500 keys x 64, one token: 30 us, 0.63 of the copy rate; one query, one key: 6.4 - 6.8 us, the launch.
 #include "attn.cuh"
 
 namespace nd {
@@ -92,15 +92,28 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas<R>) attn_few_kernel(cons
   const T* kp = static_cast<const T*>(a.k) + b * a.st[3] + h * a.st[5] + piece * 8;
   const T* vp = static_cast<const T*>(a.v) + b * a.st[6] + h * a.st[8] + piece * 8;
   const unsigned char* mask = a.mask.key_mask != nullptr ? a.mask.key_mask + static_cast<long long>(b) * a.s.sk : nullptr;
-  float m[R], l[R];
+  // With one or two rows the R x kFewUnroll scores of a step lie spread over the LPK lanes: value i (row i / kFewUnroll, key
+  // i % kFewUnroll) with the lanes of group i / kOwn, so a sum over the lanes is a few exchanges and a lane works out its own
+  // weights only (2 x 8 heads x 50021 keys of 128, one row: 72 us, 78 with every weight on every lane; two rows: 76.5 / 77.2).
+  // With four rows independent sums hide one another's latency and the longer chain costs more than it saves (four rows there:
+  // 166 us against 139): every lane has all of them. Running maximum and sum are those of a lane's own values.
+  constexpr int kVals = R * kFewUnroll, kGroups = R > 2 ? 1 : kVals < LPK ? kVals : LPK;
+  constexpr int kOwn = kVals / kGroups, kRep = LPK / kGroups;                    // values per lane, lanes with the same ones
+  constexpr int kOwnRows = kOwn > kFewUnroll ? kOwn / kFewUnroll : 1, kOwnKeys = kOwn / kOwnRows;
+  constexpr int kRowLanes = kRep * (kFewUnroll / kOwnKeys);                      // lanes that share a row
+  const int key0 = piece / kRep * kOwn % kFewUnroll;
+  auto of_group = [](float x, int g) { return kGroups == 1 ? x : __shfl_sync(0xffffffffu, x, g * kRep, LPK); };
+  float m[kOwnRows], l[kOwnRows];
+#pragma unroll
+  for (int i = 0; i < kOwnRows; ++i) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+  }
   uint64_t o[R][4];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    m[r] = -INFINITY;
-    l[r] = 0.f;
+  for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[r][e] = 0;
-  }
   for (int k0 = first; k0 < end; k0 += kStep * kFewUnroll) {
     uint4 kw[kFewUnroll], vw[kFewUnroll];
     bool on[kFewUnroll];
@@ -115,7 +128,7 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas<R>) attn_few_kernel(cons
       }
       if (mask != nullptr && on[u]) on[u] = __ldg(mask + key) != 0;
     }
-    float score[R][kFewUnroll];
+    float w[kVals];
 #pragma unroll
     for (int u = 0; u < kFewUnroll; ++u) {
       uint64_t kf[4];
@@ -126,33 +139,62 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas<R>) attn_few_kernel(cons
 #pragma unroll
         for (int e = 1; e < 4; ++e) x = f2_fma(q[r][e], kf[e], x);
         const float2 y = f2_unpack(x);
-        score[r][u] = y.x + y.y;
+        w[r * kFewUnroll + u] = y.x + y.y;
       }
     }
+    // sums over the lanes: as long as it has more than its own values a lane gives half of them away and keeps the other half
 #pragma unroll
-    for (int d = LPK / 2; d >= 1; d >>= 1)
+    for (int d = LPK / 2, n = kVals; d >= 1; d >>= 1) {
+      if (n > kOwn) {
+        n >>= 1;
+        const bool upper = (piece & d) != 0;
 #pragma unroll
-      for (int u = 0; u < kFewUnroll; ++u)
+        for (int i = 0; i < n; ++i) {
+          const float give = upper ? w[i] : w[n + i];
+          w[i] = (upper ? w[n + i] : w[i]) + __shfl_xor_sync(0xffffffffu, give, d);
+        }
+      } else {
 #pragma unroll
-        for (int r = 0; r < R; ++r) score[r][u] += __shfl_xor_sync(0xffffffffu, score[r][u], d);
+        for (int i = 0; i < kOwn; ++i) w[i] += __shfl_xor_sync(0xffffffffu, w[i], d);
+      }
+    }
+    unsigned keep = 0;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float top = m[r];
+    for (int u = 0; u < kFewUnroll; ++u) keep |= on[u] ? 1u << u : 0u;
+    float alpha[kOwnRows];
+    bool moved = false;
 #pragma unroll
-      for (int u = 0; u < kFewUnroll; ++u) {
-        score[r][u] = on[u] ? score[r][u] : -INFINITY;
-        top = max3(top, score[r][u], score[r][u]);
+    for (int i = 0; i < kOwnRows; ++i) {
+      float top = m[i];
+#pragma unroll
+      for (int u = 0; u < kOwnKeys; ++u) {
+        float& x = w[i * kOwnKeys + u];
+        x = keep >> (key0 + u) & 1 ? x : -INFINITY;
+        top = max3(top, x, x);
+      }
+#pragma unroll
+      for (int d = kRep; d < kRowLanes; d <<= 1) {
+        const float other = __shfl_xor_sync(0xffffffffu, top, d);
+        top = max3(top, other, other);
       }
       const float base = top == -INFINITY ? 0.f : top;
-      const float alpha = ex2_approx(m[r] - base);
-      m[r] = top;
-      l[r] *= alpha;
+      alpha[i] = ex2_approx(m[i] - base);
+      moved |= alpha[i] != 1.f;
+      m[i] = top;
+      l[i] *= alpha[i];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[r][e] = f2_mul(o[r][e], f2_pack(alpha, alpha));
+      for (int u = 0; u < kOwnKeys; ++u) {
+        float& x = w[i * kOwnKeys + u];
+        x = ex2_approx(x - base);
+        l[i] += x;
+      }
+    }
+    if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-      for (int u = 0; u < kFewUnroll; ++u) {
-        score[r][u] = ex2_approx(score[r][u] - base);
-        l[r] += score[r][u];
+      for (int r = 0; r < R; ++r) {
+        const float x = of_group(alpha[r * kFewUnroll % kOwn / kOwnKeys], r * kFewUnroll / kOwn);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[r][e] = f2_mul(o[r][e], f2_pack(x, x));
       }
     }
 #pragma unroll
@@ -160,21 +202,35 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas<R>) attn_few_kernel(cons
       uint64_t vf[4];
       unpack8<T>(on[u] ? vw[u] : make_uint4(0, 0, 0, 0), vf);  // a key that takes no part may hold NaN
 #pragma unroll
-      for (int r = 0; r < R; ++r)
+      for (int r = 0; r < R; ++r) {
+        const int i = r * kFewUnroll + u;
+        const float x = of_group(w[i % kOwn], i / kOwn);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[r][e] = f2_fma(f2_pack(score[r][u], score[r][u]), vf[e], o[r][e]);
+        for (int e = 0; e < 4; ++e) o[r][e] = f2_fma(f2_pack(x, x), vf[e], o[r][e]);
+      }
     }
+  }
+  // every lane with the maximum and the sum of every row
+#pragma unroll
+  for (int i = 0; i < kOwnRows; ++i)
+#pragma unroll
+    for (int d = kRep; d < kRowLanes; d <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
+  float rm[R], rl[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    rm[r] = of_group(m[r * kFewUnroll % kOwn / kOwnKeys], r * kFewUnroll / kOwn);
+    rl[r] = of_group(l[r * kFewUnroll % kOwn / kOwnKeys], r * kFewUnroll / kOwn);
   }
   // the slots of a warp, then the warps
 #pragma unroll
   for (int d = LPK; d < 32; d <<= 1)
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const float mo = __shfl_xor_sync(0xffffffffu, m[r], d), lo = __shfl_xor_sync(0xffffffffu, l[r], d);
-      const float top = max3(m[r], mo, mo), base = top == -INFINITY ? 0.f : top;
-      const float wa = ex2_approx(m[r] - base), wb = ex2_approx(mo - base);
-      m[r] = top;
-      l[r] = l[r] * wa + lo * wb;
+      const float mo = __shfl_xor_sync(0xffffffffu, rm[r], d), lo = __shfl_xor_sync(0xffffffffu, rl[r], d);
+      const float top = max3(rm[r], mo, mo), base = top == -INFINITY ? 0.f : top;
+      const float wa = ex2_approx(rm[r] - base), wb = ex2_approx(mo - base);
+      rm[r] = top;
+      rl[r] = rl[r] * wa + lo * wb;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         o[r][e] = f2_fma(__shfl_xor_sync(0xffffffffu, o[r][e], d), f2_pack(wb, wb), f2_mul(o[r][e], f2_pack(wa, wa)));
@@ -185,8 +241,8 @@ __global__ void __launch_bounds__(kFewThreads, kFewCtas<R>) attn_few_kernel(cons
 #pragma unroll
       for (int e = 0; e < 4; ++e) *reinterpret_cast<float2*>(&sh_o[warp][r][piece * 8 + 2 * e]) = f2_unpack(o[r][e]);
       if (piece == 0) {
-        sh_m[warp][r] = m[r];
-        sh_l[warp][r] = l[r];
+        sh_m[warp][r] = rm[r];
+        sh_l[warp][r] = rl[r];
       }
     }
   }
@@ -250,22 +306,23 @@ template <typename T> __global__ void __launch_bounds__(kFewThreads) attn_few_jo
 }
 
 // ------------------------------------------------------------------ host side
-// Up to two rows always (one row: 76 us against 91 us of the tile kernel at 2 x 8 heads x 50021 keys of 128, 34 against 59
+// Up to two rows always (one row: 72 us against 91 us of the tile kernel at 2 x 8 heads x 50021 keys of 128, 30 against 59
 // at 32 x 20 x 750 x 64; two rows: 76 / 90 and 27 / 59). With three or four the arithmetic counts: short keys only (32 x 16
-// x 77 x 72, four rows: 12.7 us against 19.1, 64 x 4 x 300 x 64: 11.9 / 18.7; but 64 x 16 x 300 x 128, three rows: 68 / 56,
-// 2 x 8 x 50021 x 128, four rows: 139 / 90).
+// x 77 x 72, four rows: 12.7 us against 19.1, 64 x 4 x 300 x 64: 11.9 / 18.7; but 64 x 16 x 300 x 128, three queries: 67 / 60,
+// 2 x 8 x 50021 x 128, four rows: 139 / 94) - unless the heads that share a key head do not pack into one tile (three of
+// them): there the tile kernel reads the keys once per head (2 x 8 x 50021 x 128: 139 / 248, 32 x 8 x 3000 x 64: 53 / 136).
 bool attn_few_takes(const AttnShape& s) {
   const int group = s.hq / s.hkv;
   if (s.sq > kFewRows || group > kFewRows || s.sq * group > kFewRows) return false;
-  return s.sq * group <= 2 || static_cast<long long>(s.sk) * s.d <= 32768;
+  return s.sq * group <= 2 || s.gp < group || static_cast<long long>(s.sk) * s.d <= 32768;
 }
 
 static int few_splits(const AttnShape& s, bool varies) {
   // CTAs run in rounds of what the GPU holds at once. Less than half a round: as many ranges as fill one (2 x 8 key heads x
-  // 50021 keys: 98 us with 1.1 rounds, 76 us with one), none below 64 keys. More: the fewest ranges of 512 keys and more that
+  // 50021 keys: 1.3 times as long with 1.1 rounds as with one), none below 64 keys. More: the fewest ranges of 512 keys and more that
   // fill four fifths of their rounds, else the best filled; shorter ranges do not pay for the second kernel (64 x 4 x 300
   // keys: 16 us in three ranges, 12 in one). Where lengths differ the longest sample's CTA would be the last one running:
-  // a round and a quarter of ranges, none below 256 keys (32 x 20 x up to 1500 keys: 42 us in one range, 31 in two).
+  // a round and a quarter of ranges, none below 256 keys (32 x 20 x up to 1500 keys: a third longer in one range than in two).
   const int rows = s.sq * (s.hq / s.hkv), ctas = rows == 1 ? kFewCtas<1> : rows == 2 ? kFewCtas<2> : kFewCtas<4>;
   const long long pairs = static_cast<long long>(s.batch) * s.hkv, room = static_cast<long long>(ctas) * sm_count();
   const long long most = s.sk / 64 > 1 ? s.sk / 64 : 1;

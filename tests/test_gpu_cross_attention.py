@@ -400,3 +400,22 @@ def test_refusals():
         ops.fused_cross_attention(q.cpu(), k, v)
     from novadit_b200 import capi
     assert capi.lib().nd_device_error(0) == 0
+
+
+@pytest.mark.parametrize("kind", ["none", "holes", "lens32"])
+@pytest.mark.parametrize("d", [8, 16, 24, 32, 64, 72, 128])
+@pytest.mark.parametrize("n,h,hk", [(1, 2, 2), (1, 4, 2), (2, 2, 2), (1, 6, 2), (3, 1, 1), (1, 4, 1)])
+def test_few_rows_of_every_head_size(kind, d, n, h, hk):
+    """One to four query rows per key head, heads of three sharing among them; later keys score higher, so that the maximum
+    moves all along."""
+    b, m = 3, 1100
+    dtype = torch.bfloat16 if n * h % 3 else torch.float16
+    q, k, v, dout = make(b, n, m, h, hk, d, dtype, 21)
+    k = (k.float() * torch.linspace(0.2, 2.0, m, device=DEV)[None, :, None, None]).to(dtype)
+    key_mask, kv_lens, keep = masks(kind, b, m) if kind != "none" else (None, None, None)
+    # fp16: most weights are small here and eight products hide little, so the rounding of dS below fp16's normal numbers
+    # shows. The largest |dO| of the rows goes to 2^-4 or a little below 2^-3 (see above): half of fp16's smallest number,
+    # 2^-25, is at most 2^-21 of that |dO| before the power of two is taken back.
+    tiny_s = 2.0 ** -21 * float(dout.abs().max()) if dtype == torch.float16 else None
+    want, bars = exact(q, k, v, dout, keep, 1 / math.sqrt(d), tiny_s)
+    check(run(q, k, v, dout, key_mask=key_mask, kv_lens=kv_lens), want, bars)
